@@ -48,6 +48,8 @@ enum {
 
 /* Same numeric values as GGML_TYPE_F32 / GGML_TYPE_F16. */
 enum { KK_DTYPE_F32 = 0, KK_DTYPE_F16 = 1 };
+/* Same numeric value as GGML_TYPE_BF16; only the serving operators take it. */
+enum { KK_DTYPE_BF16 = 30 };
 
 /* One weight tensor as the reference's loader holds it: logical GGUF name
  * (tools/convert_kokoro_to_gguf.py layout, dims already reversed to ggml
@@ -411,6 +413,104 @@ int kk_vocos_forward(kk_ctx *ctx, const char *prefix, const kk_vocos_params *par
 int kk_vocos_forward_device(kk_ctx *ctx, const char *prefix, const kk_vocos_params *params, int32_t n_chunks,
                             const int32_t *n_frames, const float *mel, const float *noise, float *audio,
                             void *stream);
+
+/* ---- Serving operators of a token model ----
+ * One step of a text model that feeds the synthesis front end token by
+ * token, for many requests at once (no counterpart in the reference): pages
+ * and slots of the step's new tokens, their keys and values into a paged
+ * cache, the attention of the new tokens over it, and the products with
+ * 4-bit weights around it. Device pointers, asynchronous on `stream` (NULL =
+ * the context's stream; the legacy default stream is cudaStreamLegacy, the
+ * handle 1). The lengths stay on the device, so a step needs no copy to the
+ * host. Calls without a workspace are ordered by their stream alone, unlike
+ * the calls above, and may be captured into a graph; kk_paged_attention_device
+ * says when it uses the context's.
+ *
+ * A layer's cache: value d of head h of token i of page p is
+ * k[p * page_stride + i * token_stride + h * head_stride + d] (and v with the
+ * same strides), so [page][token][head][d] and [page][head][token][d] are
+ * both served. k and v are 16-byte aligned, the strides multiples of 8
+ * values, head_dim a multiple of 8 up to KK_PAGED_MAX_HEAD_DIM. A slot is
+ * page * page_size + token. */
+#define KK_PAGED_MAX_HEAD_DIM 128
+typedef struct kk_paged_cache {
+    void *k, *v;
+    int32_t dtype; /* KK_DTYPE_F16 or KK_DTYPE_BF16 */
+    int32_t n_kv_heads, head_dim, page_size;
+    int64_t n_pages;
+    int64_t page_stride, token_stride, head_stride; /* in values */
+} kk_paged_cache;
+
+/* Pages and slots of a step. Request r has ctx_len[r] tokens in the cache and
+ * takes new_len[r] more (0 is allowed; negative counts as 0). Where its pages
+ * do not hold them it gets further ones from free_pages, the requests in
+ * order, beginning at free_pages[free_range[0]] and ending before
+ * free_range[1] (and n_free); once they run out, -1.
+ *   table      [n_seqs][max_pages] pages of each request; read below
+ *              ceil(ctx_len / page_size), the new entries written, others left
+ *   seq_len    [n_seqs] = ctx_len + new_len
+ *   cu_new     [n_seqs + 1] first new token of each request, then their number
+ *   slots      [n_tokens] slot of each new token, requests one after another;
+ *              -1 without a page (none left, or past max_pages)
+ *   positions  [n_tokens] position of each new token in its request (may be
+ *              NULL)
+ *   status     [3] the free range that is left (two values, as free_range of
+ *              the next call) and how many pages were missing; must not
+ *              overlap free_range
+ * n_tokens is at least the number of new tokens: rows of slots and positions
+ * past it are set to -1, tokens past n_tokens get neither slots nor pages in
+ * the table (though status counts their pages). */
+int kk_page_tables_device(kk_ctx *ctx, int32_t n_seqs, int32_t page_size, int32_t max_pages, const int32_t *ctx_len,
+                          const int32_t *new_len, const int32_t *free_pages, int32_t n_free,
+                          const int32_t *free_range, int32_t *table, int32_t *seq_len, int32_t *cu_new,
+                          int64_t n_tokens, int64_t *slots, int32_t *positions, int32_t *status, void *stream);
+
+/* Writes row t of k and v ([n_kv_heads][head_dim] values of `dtype`, rows
+ * k_stride and v_stride values apart, 16-byte aligned) to slot slots[t] of the
+ * cache, rounded to its type. Rows whose slot is outside the cache (-1) are
+ * skipped. Slots of one call are distinct. k and v do not overlap the cache. */
+int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_tokens, const int64_t *slots,
+                           int32_t dtype, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                           void *stream);
+
+/* Attention of the new tokens over the cache, which holds them already.
+ * seq_len, cu_new and table as kk_page_tables_device writes them; q and out
+ * [n_tokens][n_heads][head_dim] of the cache's type, rows q_stride and
+ * out_stride values apart (16-byte aligned, multiples of 8). New token t of
+ * request r is at position p = seq_len[r] - (its new tokens) + t and attends
+ * to positions 0 .. p, with window > 0 to the last `window` of them; query
+ * head h reads key head h / (n_heads / n_kv_heads).
+ *   out = softmax over j of (scale q . k_j) applied to v_j
+ * Positions without a page (a table entry outside the cache, or past
+ * max_pages) count as masked; a query that sees nothing gives 0. Masked
+ * scores and the values of tokens that no query of a request sees may be
+ * anything, NaN included; a NaN or infinite value of a token that one query
+ * sees can reach earlier queries of the same chunk. Scores, sums and maxima
+ * are 32-bit; the softmax weights are rounded to the cache's type for the
+ * product with v.
+ *   max_new, max_len: the largest number of new tokens and of cached tokens
+ * of a request. They choose how the work is divided; results are right for
+ * any values. Rows of out past the last new token are left as they were.
+ * Few rows over a long cache are worked on in pieces through a workspace of
+ * the context: such a call is ordered after the context's previous call, like
+ * the other entry points. While the stream is being captured the keys are
+ * not divided. */
+int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t n_seqs, const int32_t *seq_len,
+                              const int32_t *cu_new, int64_t n_tokens, int32_t max_new, int32_t max_len,
+                              const int32_t *table, int32_t max_pages, const void *q, int64_t q_stride,
+                              int32_t n_heads, float scale, int32_t window, void *out, int64_t out_stride,
+                              void *stream);
+
+/* out[r][n] = sum over k of x[r][k] * (q[n][k] - 8) * scales[n][k / group]
+ * (+ bias[n]), for a few rows (1 to about 16: more rows read the weights
+ * again). w: [n_out][n_in / 2] bytes, element 2 i in the low nibble of byte i
+ * and 2 i + 1 in the high one; scales: IEEE half [n_out][n_in / group]; group
+ * 32, 64 or 128, n_in a multiple of it; x and out of `dtype` (F32, F16 or
+ * BF16), rows x_stride and out_stride values apart, w and the rows of x
+ * 16-byte aligned; bias F32 or NULL. Products are exact and sums 32-bit. */
+int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in, int32_t group, const uint8_t *w,
+                        const uint16_t *scales, int32_t dtype, const void *x, int64_t x_stride, const float *bias,
+                        void *out, int64_t out_stride, void *stream);
 
 /* kk_istft without any device allocation (no counterpart in the reference,
  * whose iSTFT runs on the host). Same arguments and results as kk_istft, but

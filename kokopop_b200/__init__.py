@@ -24,6 +24,13 @@ KK_ERROR_IO = 2
 KK_ERROR_MODEL = 3
 KK_ERROR_INFERENCE = 5
 
+# tensor types (KK_DTYPE_*); BF16 for the serving operators only
+DTYPE_F32 = 0
+DTYPE_F16 = 1
+DTYPE_BF16 = 30
+# `stream` of a *_device call for the legacy default stream (0 is the context's own)
+STREAM_LEGACY = 1
+
 _f32p = ctypes.POINTER(ctypes.c_float)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
@@ -57,6 +64,23 @@ class VocosParams(ctypes.Structure):
     def of(cls, d: Dict) -> "VocosParams":
         return cls(*(int(d[n]) for n in ("dim", "blocks", "pw_hidden", "dw_kernel", "embed_kernel", "noise_ch",
                                          "mels", "n_fft", "hop")), float(d["dc_pole"]), float(d["mag_clip"]))
+
+
+class PagedCache(ctypes.Structure):
+    """kk_paged_cache: one layer's key and value pages on the device. Strides
+    in values; by default [page][token][head][head_dim] contiguous."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "n_kv_heads", "head_dim", "page_size")] + \
+               [(n, ctypes.c_int64) for n in ("n_pages", "page_stride", "token_stride", "head_stride")]
+
+    def __init__(self, k_ptr: int, v_ptr: int, dtype: int, n_pages: int, page_size: int, n_kv_heads: int,
+                 head_dim: int, page_stride: Optional[int] = None, token_stride: Optional[int] = None,
+                 head_stride: Optional[int] = None):
+        head_stride = head_dim if head_stride is None else head_stride
+        token_stride = n_kv_heads * head_dim if token_stride is None else token_stride
+        page_stride = page_size * n_kv_heads * head_dim if page_stride is None else page_stride
+        super().__init__(k_ptr, v_ptr, dtype, n_kv_heads, head_dim, page_size, n_pages, page_stride, token_stride,
+                         head_stride)
 
 
 class ProfileRecord(ctypes.Structure):
@@ -140,6 +164,12 @@ def load_library():
                                           vp, vp, vp, vp]
     L.kk_profile_records.argtypes = [vp, ctypes.POINTER(ProfileRecord), ctypes.c_size_t,
                                      ctypes.POINTER(ctypes.c_size_t)]
+    i32, i64, cachep = ctypes.c_int32, ctypes.c_int64, ctypes.POINTER(PagedCache)
+    L.kk_page_tables_device.argtypes = [vp, i32, i32, i32, vp, vp, vp, i32, vp, vp, vp, vp, i64, vp, vp, vp, vp]
+    L.kk_cache_append_device.argtypes = [vp, cachep, i64, vp, i32, vp, i64, vp, i64, vp]
+    L.kk_paged_attention_device.argtypes = [vp, cachep, i32, vp, vp, i64, i32, i32, vp, i32, vp, i64, i32,
+                                            ctypes.c_float, i32, vp, i64, vp]
+    L.kk_q4_matvec_device.argtypes = [vp, i64, i32, i32, i32, vp, vp, i32, vp, i64, vp, vp, i64, vp]
     i64p = ctypes.POINTER(ctypes.c_int64)
     cfgp = ctypes.POINTER(StreamConfig)
     L.kk_stream_preset.argtypes = [ctypes.c_int32, cfgp]
@@ -373,6 +403,39 @@ class Context:
         audio = np.zeros(max(1, (n - 1) * 5), np.float32)
         self._check(self.L.kk_istft(self.h, n, _ptr(post), _ptr(audio)))
         return audio[: max(0, (n - 1) * 5)]
+
+    # ---- serving operators of a token model (device pointers, asynchronous) ----
+
+    def page_tables_device(self, n_seqs: int, page_size: int, max_pages: int, ctx_len_ptr: int, new_len_ptr: int,
+                           free_pages_ptr: int, n_free: int, free_range_ptr: int, table_ptr: int, seq_len_ptr: int,
+                           cu_new_ptr: int, n_tokens: int, slots_ptr: int, positions_ptr: int, status_ptr: int,
+                           stream: int = 0) -> None:
+        """kk_page_tables_device: int32 throughout but the int64 slots."""
+        self._check(self.L.kk_page_tables_device(self.h, n_seqs, page_size, max_pages, ctx_len_ptr, new_len_ptr,
+                                                 free_pages_ptr, n_free, free_range_ptr, table_ptr, seq_len_ptr,
+                                                 cu_new_ptr, n_tokens, slots_ptr, positions_ptr, status_ptr, stream))
+
+    def cache_append_device(self, cache: PagedCache, n_tokens: int, slots_ptr: int, dtype: int, k_ptr: int,
+                            k_stride: int, v_ptr: int, v_stride: int, stream: int = 0) -> None:
+        """kk_cache_append_device: k, v rows [n_kv_heads, head_dim] of `dtype`, strides in values."""
+        self._check(self.L.kk_cache_append_device(self.h, cache, n_tokens, slots_ptr, dtype, k_ptr, k_stride, v_ptr,
+                                                  v_stride, stream))
+
+    def paged_attention_device(self, cache: PagedCache, n_seqs: int, seq_len_ptr: int, cu_new_ptr: int, n_tokens: int,
+                               max_new: int, max_len: int, table_ptr: int, max_pages: int, q_ptr: int, q_stride: int,
+                               n_heads: int, scale: float, window: int, out_ptr: int, out_stride: int,
+                               stream: int = 0) -> None:
+        """kk_paged_attention_device: q, out rows [n_heads, head_dim] of the cache's type, strides in values."""
+        self._check(self.L.kk_paged_attention_device(self.h, cache, n_seqs, seq_len_ptr, cu_new_ptr, n_tokens,
+                                                     max_new, max_len, table_ptr, max_pages, q_ptr, q_stride, n_heads,
+                                                     scale, window, out_ptr, out_stride, stream))
+
+    def q4_matvec_device(self, n_rows: int, n_out: int, n_in: int, group: int, w_ptr: int, scales_ptr: int,
+                         dtype: int, x_ptr: int, x_stride: int, bias_ptr: int, out_ptr: int, out_stride: int,
+                         stream: int = 0) -> None:
+        """kk_q4_matvec_device: x [n_rows, n_in], out [n_rows, n_out] of `dtype`; bias_ptr 0: none."""
+        self._check(self.L.kk_q4_matvec_device(self.h, n_rows, n_out, n_in, group, w_ptr, scales_ptr, dtype, x_ptr,
+                                               x_stride, bias_ptr, out_ptr, out_stride, stream))
 
     # ---- LSTM stack and durations ----
 

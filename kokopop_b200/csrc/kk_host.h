@@ -234,3 +234,45 @@ struct kk_ctx {
     const kk::LstmLayer &lstm_layer(const std::string &prefix);
     const kk::VocosNet &vocos_net(const std::string &prefix, const kk_vocos_params &p);
 };
+
+namespace kk {
+
+// Runs an entry point's body: a C++ exception becomes its status and the
+// message of kk_last_error().
+template <typename F>
+int guarded(F &&f) noexcept {
+    try {
+        return f();
+    } catch (const KKError &e) {
+        set_last_error(e.what());
+        return e.code;
+    } catch (const std::exception &e) {
+        set_last_error(e.what());
+        return KK_ERROR_INFERENCE;
+    } catch (...) {
+        set_last_error("unknown C++ exception");
+        return KK_ERROR_INFERENCE;
+    }
+}
+
+inline void use_device(kk_ctx *ctx) { check_cuda(cudaSetDevice(ctx->device), "cudaSetDevice"); }
+
+// Brackets one entry point's work on `st`: orders it after the context's
+// previous call, which may have run on another stream and whose workspaces
+// this call reuses, and opens a pinned staging slot for its small uploads.
+struct CallScope {
+    kk_ctx &c;
+    cudaStream_t st;
+    CallScope(kk_ctx &ctx, cudaStream_t s) : c(ctx), st(s) {
+        if (c.done_recorded) check_cuda(cudaStreamWaitEvent(st, c.ev_done, 0), "order after the previous call");
+        c.stage_begin();
+    }
+    ~CallScope() {
+        c.done_recorded = cudaEventRecord(c.ev_done, st) == cudaSuccess;
+        if (!c.done_recorded) cudaStreamSynchronize(st);  // nothing to wait for next time
+    }
+    CallScope(const CallScope &) = delete;
+    CallScope &operator=(const CallScope &) = delete;
+};
+
+}  // namespace kk

@@ -355,4 +355,77 @@ void duration_frames(const float *d, int64_t n, float speed, int32_t *frames, in
 void align_gather(const float *hidden, int64_t D, const int32_t *frames, const int64_t *start, int64_t n, float *en,
                   cudaStream_t st);
 
+// ---- serving operators of a token model ----
+// A layer's paged cache as the kernels take it: token i of page p, head h
+// begins p * page_stride + i * token_stride + h * head_stride values after k
+// (and v). 16-bit values.
+struct PagedCacheView {
+    void *k, *v;
+    int bf16;  // values are bfloat16, else half
+    int n_kv_heads, head_dim, page_size;
+    int64_t n_pages, page_stride, token_stride, head_stride;
+};
+
+// kk_paged.cu
+struct PageTablesArgs {
+    int n_seqs, page_size, max_pages;
+    const int32_t *ctx_len, *new_len;
+    const int32_t *free_pages;
+    int64_t free_cap;
+    const int32_t *free_range;
+    int32_t *table, *seq_len, *cu_new;
+    int64_t n_tokens;
+    int64_t *slots;
+    int32_t *positions;  // may be null
+    int32_t *status;
+};
+cudaError_t page_tables(const PageTablesArgs &a, cudaStream_t st);
+
+struct CacheAppendArgs {
+    PagedCacheView cache;
+    int64_t n_tokens;
+    const int64_t *slots;
+    int dtype;  // KK_DTYPE_* of k and v
+    const void *k, *v;
+    int64_t k_stride, v_stride;
+};
+cudaError_t cache_append(const CacheAppendArgs &a, cudaStream_t st);
+
+// kk_paged_attn.cu
+struct PagedAttnArgs {
+    PagedCacheView cache;
+    int n_seqs, n_heads, max_pages;
+    const int32_t *seq_len, *cu_new, *table;
+    int64_t n_tokens;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    float scale;
+    int window;  // 0: none
+    // the key axis in `splits` pieces of at least split_keys keys (see there)
+    int splits, split_keys;
+    float *part_o;   // [n_tokens][n_heads][splits][head_dim]
+    float2 *part_ml; // [n_tokens][n_heads][splits] running maximum (base 2) and sum
+    unsigned *count; // [row tiles][n_kv_heads], zero between launches
+};
+// row tiles of the kernel: at most this many for n_tokens tokens of n_seqs
+// requests, `group` query heads on each key head
+int64_t paged_attn_tiles(int64_t n_tokens, int n_seqs, int group);
+cudaError_t paged_attn(const PagedAttnArgs &a, cudaStream_t st);
+
+// kk_q4.cu
+struct Q4MatvecArgs {
+    int64_t n_rows;
+    int n_out, n_in, group;
+    const uint8_t *w;
+    const __half *scales;
+    int dtype;  // KK_DTYPE_* of x and out
+    const void *x;
+    int64_t x_stride;
+    const float *bias;  // may be null
+    void *out;
+    int64_t out_stride;
+};
+cudaError_t q4_matvec(const Q4MatvecArgs &a, cudaStream_t st);
+
 }  // namespace kk

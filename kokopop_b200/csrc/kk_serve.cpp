@@ -1,0 +1,239 @@
+// C ABI of the serving operators of a token model (include/kokopop_b200.h):
+// argument checks, workspaces and launches.
+#include "kk_host.h"
+
+#include <algorithm>
+#include <cstdint>
+
+using namespace kk;
+
+namespace {
+
+[[noreturn]] void invalid(const std::string &m) { throw KKError(KK_ERROR_INVALID_ARGUMENT, m); }
+
+void need(bool ok, const char *m) {
+    if (!ok) invalid(m);
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+bool dtype16(int dtype) { return dtype == KK_DTYPE_F16 || dtype == KK_DTYPE_BF16; }
+bool dtype_any(int dtype) { return dtype == KK_DTYPE_F32 || dtype16(dtype); }
+
+constexpr int64_t kMaxTokens = INT32_MAX / 2;  // rows of one call
+
+PagedCacheView cache_view(const kk_paged_cache *c) {
+    need(c && c->k && c->v, "null cache");
+    need(dtype16(c->dtype), "cache dtype is not F16 or BF16");
+    need(c->n_kv_heads >= 1 && c->n_kv_heads <= 65535, "cache n_kv_heads out of range [1, 65535]");
+    need(c->head_dim >= 8 && c->head_dim <= KK_PAGED_MAX_HEAD_DIM && c->head_dim % 8 == 0,
+         "cache head_dim is not a multiple of 8 in [8, 128]");
+    need(c->page_size >= 1 && c->n_pages >= 1 && c->n_pages <= INT32_MAX, "cache page_size or n_pages out of range");
+    need(aligned16(c->k) && aligned16(c->v), "cache k and v must be 16-byte aligned");
+    need(c->page_stride >= 0 && c->token_stride >= 0 && c->head_stride >= 0 && c->page_stride % 8 == 0 &&
+             c->token_stride % 8 == 0 && c->head_stride % 8 == 0,
+         "cache strides must be multiples of 8 values");
+    PagedCacheView v;
+    v.k = c->k;
+    v.v = c->v;
+    v.bf16 = c->dtype == KK_DTYPE_BF16;
+    v.n_kv_heads = c->n_kv_heads;
+    v.head_dim = c->head_dim;
+    v.page_size = c->page_size;
+    v.n_pages = c->n_pages;
+    v.page_stride = c->page_stride;
+    v.token_stride = c->token_stride;
+    v.head_stride = c->head_stride;
+    return v;
+}
+
+cudaStream_t stream_of(kk_ctx *ctx, void *stream) { return stream ? (cudaStream_t)stream : ctx->st; }
+
+bool capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &s) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream while another one captures
+        return false;
+    }
+    return s != cudaStreamCaptureStatusNone;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kk_page_tables_device(kk_ctx *ctx, int32_t n_seqs, int32_t page_size, int32_t max_pages, const int32_t *ctx_len,
+                          const int32_t *new_len, const int32_t *free_pages, int32_t n_free,
+                          const int32_t *free_range, int32_t *table, int32_t *seq_len, int32_t *cu_new,
+                          int64_t n_tokens, int64_t *slots, int32_t *positions, int32_t *status, void *stream) {
+    return guarded([&] {
+        need(ctx && ctx_len && new_len && free_range && table && seq_len && cu_new && status, "null argument");
+        need(n_seqs >= 1 && page_size >= 1 && max_pages >= 1, "n_seqs, page_size or max_pages below 1");
+        need(n_free >= 0 && (free_pages || n_free == 0), "null free_pages or negative n_free");
+        need(n_tokens >= 0 && n_tokens <= kMaxTokens && (slots || n_tokens == 0), "null slots or n_tokens out of range");
+        need((uintptr_t)(free_range + 2) <= (uintptr_t)status || (uintptr_t)(status + 3) <= (uintptr_t)free_range,
+             "status overlaps free_range");
+        use_device(ctx);
+        PageTablesArgs a;
+        a.n_seqs = n_seqs;
+        a.page_size = page_size;
+        a.max_pages = max_pages;
+        a.ctx_len = ctx_len;
+        a.new_len = new_len;
+        a.free_pages = free_pages;
+        a.free_cap = n_free;
+        a.free_range = free_range;
+        a.table = table;
+        a.seq_len = seq_len;
+        a.cu_new = cu_new;
+        a.n_tokens = n_tokens;
+        a.slots = slots;
+        a.positions = positions;
+        a.status = status;
+        check_cuda(page_tables(a, stream_of(ctx, stream)), "page tables launch");
+        ++ctx->n_launches;
+        return KK_OK;
+    });
+}
+
+int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_tokens, const int64_t *slots,
+                           int32_t dtype, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                           void *stream) {
+    return guarded([&] {
+        need(ctx != nullptr, "null argument");
+        CacheAppendArgs a;
+        a.cache = cache_view(cache);
+        need(n_tokens >= 0 && n_tokens <= kMaxTokens, "n_tokens out of range");
+        need(dtype_any(dtype), "dtype is not F32, F16 or BF16");
+        if (n_tokens == 0) return KK_OK;
+        need(slots && k && v, "null argument");
+        const int64_t row = (int64_t)a.cache.n_kv_heads * a.cache.head_dim, step = dtype == KK_DTYPE_F32 ? 4 : 8;
+        need(aligned16(k) && aligned16(v), "k and v must be 16-byte aligned");
+        need(k_stride >= row && v_stride >= row && k_stride % step == 0 && v_stride % step == 0,
+             "k and v strides must hold a row and be multiples of 16 bytes");
+        use_device(ctx);
+        a.n_tokens = n_tokens;
+        a.slots = slots;
+        a.dtype = dtype;
+        a.k = k;
+        a.v = v;
+        a.k_stride = k_stride;
+        a.v_stride = v_stride;
+        check_cuda(cache_append(a, stream_of(ctx, stream)), "cache append launch");
+        ++ctx->n_launches;
+        return KK_OK;
+    });
+}
+
+int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t n_seqs, const int32_t *seq_len,
+                              const int32_t *cu_new, int64_t n_tokens, int32_t max_new, int32_t max_len,
+                              const int32_t *table, int32_t max_pages, const void *q, int64_t q_stride,
+                              int32_t n_heads, float scale, int32_t window, void *out, int64_t out_stride,
+                              void *stream) {
+    return guarded([&] {
+        need(ctx != nullptr, "null argument");
+        PagedAttnArgs a;
+        a.cache = cache_view(cache);
+        need(seq_len && cu_new && table, "null argument");
+        need(n_seqs >= 1 && max_pages >= 1 && max_new >= 0 && max_len >= 0,
+             "n_seqs or max_pages below 1, or a negative max_new or max_len");
+        need(n_tokens >= 0 && n_tokens <= kMaxTokens, "n_tokens out of range");
+        need(n_heads >= 1 && n_heads % a.cache.n_kv_heads == 0, "n_heads is not a multiple of the cache's n_kv_heads");
+        need(scale == scale, "scale is not a number");
+        need(window >= 0, "negative window");
+        if (n_tokens == 0) return KK_OK;
+        need(q && out, "null argument");
+        const int64_t row = (int64_t)n_heads * a.cache.head_dim;
+        need(aligned16(q) && aligned16(out), "q and out must be 16-byte aligned");
+        need(q_stride >= row && out_stride >= row && q_stride % 8 == 0 && out_stride % 8 == 0,
+             "q and out strides must hold a row and be multiples of 8 values");
+        const int group = n_heads / a.cache.n_kv_heads;
+        const int64_t tiles = paged_attn_tiles(n_tokens, n_seqs, group);
+        need(tiles <= INT32_MAX && n_tokens * group <= INT32_MAX, "n_tokens x query heads per key head out of range");
+        use_device(ctx);
+        cudaStream_t st = stream_of(ctx, stream);
+        a.n_seqs = n_seqs;
+        a.n_heads = n_heads;
+        a.max_pages = max_pages;
+        a.seq_len = seq_len;
+        a.cu_new = cu_new;
+        a.table = table;
+        a.n_tokens = n_tokens;
+        a.q = q;
+        a.out = out;
+        a.q_stride = q_stride;
+        a.out_stride = out_stride;
+        a.scale = scale;
+        a.window = window;
+        a.part_o = nullptr;
+        a.part_ml = nullptr;
+        a.count = nullptr;
+        // pieces of the key axis: enough blocks for about four rounds of two
+        // blocks on each of 148 SMs, 128 keys or more each
+        const int64_t most_rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
+        const int64_t blocks = std::min(tiles, n_seqs * ((most_rows + 15) / 16)) * a.cache.n_kv_heads;
+        int64_t keys = std::max(max_len, 1);
+        if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + 16);
+        const int64_t splits = std::min((1184 + blocks - 1) / blocks, (keys + 127) / 128);
+        a.splits = capturing(st) ? 1 : (int)std::min<int64_t>(splits, 256);
+        a.split_keys = (int)(((keys + a.splits - 1) / a.splits + 63) / 64 * 64);
+        if (a.splits == 1) {
+            check_cuda(paged_attn(a, st), "paged attention launch");
+            ++ctx->n_launches;
+            return KK_OK;
+        }
+        CallScope call_scope(*ctx, st);
+        const size_t parts = (size_t)n_tokens * n_heads * a.splits;
+        a.part_o = ctx->buf("paged_part_o", parts * a.cache.head_dim);
+        a.part_ml = (float2 *)ctx->buf("paged_part_ml", parts * 2);
+        DevBuf &count = ctx->ws["paged_count"];
+        const size_t count_bytes = (size_t)tiles * a.cache.n_kv_heads * sizeof(unsigned);
+        if (count.bytes < count_bytes) {
+            count.ensure(count_bytes);
+            check_cuda(cudaMemsetAsync(count.p, 0, count.bytes, st), "clear the piece counters");
+        }
+        a.count = (unsigned *)count.p;
+        check_cuda(paged_attn(a, st), "paged attention launch");
+        ++ctx->n_launches;
+        return KK_OK;
+    });
+}
+
+int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in, int32_t group, const uint8_t *w,
+                        const uint16_t *scales, int32_t dtype, const void *x, int64_t x_stride, const float *bias,
+                        void *out, int64_t out_stride, void *stream) {
+    return guarded([&] {
+        need(ctx && w && scales, "null argument");
+        need(n_rows >= 0 && n_rows <= 8 * 65535 && n_out >= 1 && n_in >= 1, "n_rows, n_out or n_in out of range");
+        need(group == 32 || group == 64 || group == 128, "group is not 32, 64 or 128");
+        need(n_in % group == 0, "n_in is not a multiple of the group");
+        need(dtype_any(dtype), "dtype is not F32, F16 or BF16");
+        if (n_rows == 0) return KK_OK;
+        need(x && out, "null argument");
+        need(aligned16(w) && aligned16(x), "w and x must be 16-byte aligned");
+        need(((uintptr_t)scales & 1) == 0 && ((uintptr_t)bias & 3) == 0 &&
+                 ((uintptr_t)out & (dtype == KK_DTYPE_F32 ? 3 : 1)) == 0,
+             "scales, bias or out is not aligned to its type");
+        need(x_stride >= n_in && x_stride % (dtype == KK_DTYPE_F32 ? 4 : 8) == 0,
+             "x stride must hold a row and be a multiple of 16 bytes");
+        need(out_stride >= n_out, "out stride must hold a row");
+        use_device(ctx);
+        Q4MatvecArgs a;
+        a.n_rows = n_rows;
+        a.n_out = n_out;
+        a.n_in = n_in;
+        a.group = group;
+        a.w = w;
+        a.scales = (const __half *)scales;
+        a.dtype = dtype;
+        a.x = x;
+        a.x_stride = x_stride;
+        a.bias = bias;
+        a.out = out;
+        a.out_stride = out_stride;
+        check_cuda(q4_matvec(a, stream_of(ctx, stream)), "4-bit product launch");
+        ++ctx->n_launches;
+        return KK_OK;
+    });
+}
+
+}  // extern "C"
