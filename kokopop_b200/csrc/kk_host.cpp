@@ -2025,6 +2025,8 @@ void check_device_error(kk_ctx *ctx) {
     if (e == kErrLstmWait)
         throw KKError(KK_ERROR_INFERENCE, "LSTM recurrence timed out waiting for a step's hidden state (code " +
                                               std::to_string(e) + ")");
+    if (e == kErrPagedWait)
+        throw KKError(KK_ERROR_INFERENCE, "paged attention timed out waiting (code " + std::to_string(e) + ")");
     throw KKError(KK_ERROR_INFERENCE, "tensor-core convolution timed out waiting (code " + std::to_string(e) + ")");
 }
 

@@ -406,12 +406,25 @@ struct PagedAttnArgs {
     int splits, split_keys;
     float *part_o;   // [n_tokens][n_heads][splits][head_dim]
     float2 *part_ml; // [n_tokens][n_heads][splits] running maximum (base 2) and sum
-    unsigned *count; // [row tiles][n_kv_heads], zero between launches
+    unsigned *count; // [tiles][n_kv_heads], zero between launches
+    int *err;        // device error word
 };
-// row tiles of the kernel: at most this many for n_tokens tokens of n_seqs
-// requests, `group` query heads on each key head
-int64_t paged_attn_tiles(int64_t n_tokens, int n_seqs, int group);
-cudaError_t paged_attn(const PagedAttnArgs &a, cudaStream_t st);
+// How a call is divided: the tensor-memory kernel (chunks of queries) or the
+// row kernel (a few queries of each request), rows (query, head of the group)
+// of a tile, and at most how many tiles there are.
+struct PagedAttnPlan {
+    bool chunk;
+    int unit;
+    int64_t tiles;
+};
+PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new);
+cudaError_t paged_attn(const PagedAttnPlan &p, const PagedAttnArgs &a, cudaStream_t st);
+// kk_paged_chunk.cu
+bool paged_chunk_serves(const PagedCacheView &c, int n_heads);
+int paged_chunk_unit(int group);
+cudaError_t paged_chunk_attn(const PagedAttnArgs &a, cudaStream_t st);
+// A wait of the chunk kernel ran out (2 s).
+constexpr int kErrPagedWait = 78;
 
 // kk_q4.cu
 struct Q4MatvecArgs {

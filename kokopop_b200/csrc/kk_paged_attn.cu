@@ -23,8 +23,7 @@
 // are joined in shared memory, the pieces in global memory by the block that
 // arrives last, in the order of the pieces, so that the result does not
 // depend on which one that is.
-#include "kk_common.cuh"
-#include "kk_kernels.h"
+#include "kk_paged_attn.cuh"
 
 #include <atomic>
 
@@ -89,54 +88,6 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// The row tile `w` of a launch. Request r's tiles begin at
-// floor(cu[r] * group / kRows) + r: consecutive requests are at least as far
-// apart as request r has tiles, so the request is found by bisection of
-// cu_new alone, and at most paged_attn_tiles() indices are in use.
-struct RowTile {
-    int r;         // request, -1: no such tile
-    int row0;      // first row (query * group + head of the group) in the request
-    int rows;      // rows of the request
-    int64_t tok0;  // its first token's row in q and out
-    int n;         // its new tokens (those that n_tokens covers)
-    int base;      // position of its first new token
-};
-
-__device__ __forceinline__ int64_t first_tile(const PagedAttnArgs &a, int group, int r) {
-    return min((int64_t)max(a.cu_new[r], 0), a.n_tokens) * group / kRows + r;
-}
-
-__device__ __forceinline__ RowTile find_tile(const PagedAttnArgs &a, int group, int64_t w) {
-    RowTile t;
-    int x = 0, y = a.n_seqs - 1;
-    while (x < y) {
-        const int mid = (x + y + 1) >> 1;
-        if (first_tile(a, group, mid) <= w)
-            x = mid;
-        else
-            y = mid - 1;
-    }
-    t.r = x;
-    t.tok0 = min((int64_t)max(a.cu_new[x], 0), a.n_tokens);
-    const int64_t tok1 = min((int64_t)max(a.cu_new[x + 1], 0), a.n_tokens);
-    t.n = tok1 > t.tok0 ? (int)(tok1 - t.tok0) : 0;
-    t.base = a.seq_len[x] - max(a.cu_new[x + 1] - a.cu_new[x], 0);
-    const int64_t row0 = (w - first_tile(a, group, x)) * kRows, rows = (int64_t)t.n * group;
-    if (row0 < 0 || row0 >= rows) t.r = -1;
-    t.row0 = (int)row0;
-    t.rows = rows > INT32_MAX ? INT32_MAX : (int)rows;
-    return t;
-}
-
 }  // namespace
 
 template <typename T, int DP>
@@ -150,7 +101,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attn_row(PagedAttnArgs a)
     __shared__ unsigned last_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
     const int group = a.n_heads / a.cache.n_kv_heads, kvh = blockIdx.y;
-    const RowTile t = find_tile(a, group, blockIdx.x);
+    const RowTile t = find_tile(a, group, kRows, blockIdx.x);
     if (t.r < 0) return;  // the whole block
     const int D = a.cache.head_dim;
 
@@ -198,7 +149,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attn_row(PagedAttnArgs a)
     const int n_blocks = (int)((k1 - k0 + kKeys - 1) / kKeys);
     const int n_steps = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;
     unsigned char *ring = sm + warp * kStages * 2 * C::TILE;
-    const T *kc = (const T *)a.cache.k + kvh * a.cache.head_stride, *vc = (const T *)a.cache.v + kvh * a.cache.head_stride;
+    const T *kc = (const T *)a.cache.k + kvh * a.cache.head_stride;
+    const T *vc = (const T *)a.cache.v + kvh * a.cache.head_stride;
     const int32_t *table = a.table + (int64_t)t.r * a.max_pages;
 
     auto issue = [&](int s) {
@@ -373,10 +325,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attn_row(PagedAttnArgs a)
     }
 }
 
-int64_t paged_attn_tiles(int64_t n_tokens, int n_seqs, int group) { return n_tokens * group / kRows + n_seqs; }
-
 template <typename T, int DP>
-static cudaError_t launch_row(const PagedAttnArgs &a, cudaStream_t st) {
+static cudaError_t launch_row(const PagedAttnArgs &a, int64_t tiles, cudaStream_t st) {
     static std::atomic<bool> attr[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -388,16 +338,26 @@ static cudaError_t launch_row(const PagedAttnArgs &a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         attr[dev].store(true, std::memory_order_release);
     }
-    const int64_t tiles = paged_attn_tiles(a.n_tokens, a.n_seqs, a.n_heads / a.cache.n_kv_heads);
     const dim3 grid((unsigned)tiles, (unsigned)a.cache.n_kv_heads, (unsigned)a.splits);
     k_paged_attn_row<T, DP><<<grid, kWarps * 32, RowCfg<DP>::SMEM, st>>>(a);
     return cudaGetLastError();
 }
 
-cudaError_t paged_attn(const PagedAttnArgs &a, cudaStream_t st) {
+PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new) {
+    const int group = n_heads / c.n_kv_heads;
+    const int64_t rows = (n_tokens < max_new ? n_tokens : max_new) * (int64_t)group;
+    PagedAttnPlan p;
+    p.chunk = rows > kRows && paged_chunk_serves(c, n_heads);
+    p.unit = p.chunk ? paged_chunk_unit(group) : kRows;
+    p.tiles = n_tokens * group / p.unit + n_seqs;
+    return p;
+}
+
+cudaError_t paged_attn(const PagedAttnPlan &p, const PagedAttnArgs &a, cudaStream_t st) {
+    if (p.chunk) return paged_chunk_attn(a, st);
     if (a.cache.head_dim <= 64)
-        return a.cache.bf16 ? launch_row<__nv_bfloat16, 64>(a, st) : launch_row<__half, 64>(a, st);
-    return a.cache.bf16 ? launch_row<__nv_bfloat16, 128>(a, st) : launch_row<__half, 128>(a, st);
+        return a.cache.bf16 ? launch_row<__nv_bfloat16, 64>(a, p.tiles, st) : launch_row<__half, 64>(a, p.tiles, st);
+    return a.cache.bf16 ? launch_row<__nv_bfloat16, 128>(a, p.tiles, st) : launch_row<__half, 128>(a, p.tiles, st);
 }
 
 }  // namespace kk

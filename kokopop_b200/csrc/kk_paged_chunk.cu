@@ -1,0 +1,616 @@
+// Attention of chunks of new tokens over the paged cache on the 5th-generation
+// tensor cores (sm_100a); the definition is in kk_paged_attn.cu. With many
+// query rows per key head the arithmetic bounds it: 4 head_dim operations per
+// (row, key), and one exponential, of which an SM does 16 a clock.
+//
+// A block takes two tiles of up to 128 rows (query, head of the group) of one
+// key head and one piece of the key axis, 128 keys a step. The tiles take
+// turns: while the tensor cores work on one tile's products, the other's 128
+// threads (thread = row = lane of tensor memory) do its softmax, so both pipes
+// stay busy and no row needs a reduction between threads.
+//   S = Q K^T      128 x 128 x head_dim, into tensor memory
+//   P = e^(S - m)  read from, and written back over, tensor memory as 16 bits
+//   O += P V       P from tensor memory, V as it lies (keys x dims)
+// m follows the running maximum lazily: O is rescaled only when the maximum
+// has grown by more than 8 in base 2 (the weights stay below 2^8), which after
+// the first steps is rare; the result does not depend on m but for rounding.
+//
+// Roles: warps 0-3 and 4-7 softmax and output of the two tiles, warp 8 issues
+// the tcgen05.mma, warp 9 the copies (10 and 11 only fill their warpgroup). Keys and values come page by page
+// through 4-D tensor maps (dim, token, head, page) into 128-byte swizzled
+// tiles, so any stride order of the cache is served; pages that are missing or
+// hold no key of the tile are fetched from outside the tensor and read as
+// zeros. Values of tokens outside the block's key range may be anything, and 0
+// times a NaN is one: their rows are zeroed in shared memory in the steps at
+// the two ends of the range.
+//
+// The order of the MMAs is the ping-pong of the two tiles, O += P V of step j
+// followed by S = Q K^T of step j + 1. For head_dim above 64 tensor memory is
+// full (2 x 128 columns of S, 2 x 128 of O), P lies over S, and the new S has
+// to wait until the product that reads P has completed; for head_dim up to 64
+// P has columns of its own.
+#include "kk_paged_attn.cuh"
+#include "kk_ptx.cuh"
+
+#include <cudaTypedefs.h>
+
+#include <atomic>
+
+namespace kk {
+
+namespace {
+
+constexpr int kTile = 128;       // rows of a tile, keys of a step
+constexpr int kStages = 5;       // K or V tiles in flight
+constexpr int kThreads = 384;
+// registers of a thread: 168 at launch (3 warpgroups), moved from the copy and
+// MMA warpgroup to the two that hold a row of scores: 56 + 2 x 224 = 3 x 168
+constexpr int kRegsFew = 56, kRegsMany = 224;
+constexpr int kMmaWarp = 8, kCopyWarp = 9;
+constexpr float kGrow = 8.0f;    // base-2 growth of a maximum that is left alone
+
+template <int DP>
+struct ChunkCfg {
+    static constexpr int TILE_BYTES = kTile * DP * 2;
+    static constexpr int HALF_BYTES = kTile * 128;   // 64 dims of a tile
+    static constexpr int SMEM = (2 + kStages) * TILE_BYTES + 1024 /*barriers*/ + 1024 /*align*/;
+    static constexpr bool P_OVER_S = DP > 64;
+    // tensor memory columns
+    static constexpr int S0 = 0, O0 = 2 * kTile, P0 = P_OVER_S ? 0 : O0 + 2 * DP, P_STEP = P_OVER_S ? kTile : kTile / 2;
+    static constexpr int COLS = 512;
+};
+static_assert(ChunkCfg<128>::SMEM <= 227 * 1024, "shared memory");
+
+// Shared-memory matrix descriptor, 128-byte swizzle (mode 2 in [61,64)).
+__device__ __forceinline__ uint64_t sdesc128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return sdesc(addr, lbo, sbo) | (2ull << 61);
+}
+
+// Instruction descriptor, kind::f16: D F32, A and B half (0) or bfloat16 (1)
+// at bits 7 and 10, B transposed (its rows are the sum's axis) at bit 16.
+__device__ __forceinline__ constexpr uint32_t idesc_of(int bf16, int b_rows, int n) {
+    return idesc_f16(kTile, n) | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)b_rows << 16;
+}
+
+// D[tmem] (+)= A[tmem] B
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+#define KK_R32(r) \
+    "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), \
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), \
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), \
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+// 32 columns of this thread's lane, without the wait
+__device__ __forceinline__ void tmem_get32(uint32_t taddr, float *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : KK_R32(r)
+        : "r"(taddr));
+}
+#undef KK_R32
+__device__ __forceinline__ void tmem_get_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_put32(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 2^x, results below 2^-126 as 0 (a weight is at most 2^kGrow and rounded to
+// 16 bits afterwards)
+__device__ __forceinline__ float pow2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z,
+                                            int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+
+}  // namespace
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_paged_attn_chunk(PagedAttnArgs a, const __grid_constant__ CUtensorMap map_q,
+                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    using C = ChunkCfg<DP>;
+    constexpr int HALVES = DP / 64;
+    constexpr int BF16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint32_t tmem_s;
+    __shared__ unsigned last_s;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = a.n_heads / a.cache.n_kv_heads, kvh = blockIdx.y, D = a.cache.head_dim;
+    const int tile_tok = kTile / group;  // tokens of a tile
+    // the last tiles of a request see the most keys: first
+    const RowTile t = find_tile(a, group, 2 * tile_tok * group, gridDim.x - 1 - blockIdx.x);
+    if (t.r < 0) return;  // the whole block
+
+    // the tiles' tokens and key ranges, the block's piece of the keys
+    const int64_t cap = (int64_t)a.max_pages * a.cache.page_size;
+    const int tok_first = t.row0 / group;
+    int tok[2], n_tok[2], n_step[2];
+    int64_t hi[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        tok[x] = tok_first + x * tile_tok;
+        n_tok[x] = max(min(t.n - tok[x], tile_tok), 0);
+        hi[x] = n_tok[x] > 0 ? max(min((int64_t)t.base + tok[x] + n_tok[x], cap), (int64_t)0) : 0;
+    }
+    const int64_t lo = a.window > 0 ? max((int64_t)t.base + tok_first - a.window + 1, (int64_t)0) : 0;
+    const int64_t kbeg = lo / kTile * kTile, kend = max(max(hi[0], hi[1]), kbeg);
+    int64_t piece = (kend - kbeg + a.splits - 1) / a.splits;
+    piece = max((piece + kTile - 1) / kTile * kTile, (int64_t)a.split_keys);
+    const int n_pieces = (int)max((kend - kbeg + piece - 1) / piece, (int64_t)1);
+    const int sp = blockIdx.z;
+    if (sp >= n_pieces) return;
+    const int64_t k0 = kbeg + sp * piece, k1 = min(k0 + piece, kend);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) n_step[x] = (int)((max(min(k1, hi[x]) - k0, (int64_t)0) + kTile - 1) / kTile);
+    const int steps = max(n_step[0], n_step[1]);
+    const int32_t *table = a.table + (int64_t)t.r * a.max_pages;
+    const int page_size = a.cache.page_size;
+
+    uint8_t *sQ = smem, *sKV = smem + 2 * C::TILE_BYTES;
+    const uint32_t bars = smem_u32(sKV + kStages * C::TILE_BYTES);
+    const uint32_t bQ = bars, bFull = bars + 16, bEmpty = bFull + 8 * kStages, bS = bEmpty + 8 * kStages,
+                   bP = bS + 16, bPV = bP + 16, bDrain = bPV + 16;
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bQ + 8 * i, 1);
+            mbar_init(bS + 8 * i, 1);
+            mbar_init(bP + 8 * i, kTile);
+            mbar_init(bPV + 8 * i, 1);
+        }
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(bFull + 8 * i, 1);
+            mbar_init(bEmpty + 8 * i, 1);
+        }
+        mbar_init(bDrain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
+                     "r"(C::COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tmem_s;
+
+    // The roles part here for good: each side has its own register budget, and
+    // they meet once more at the block barrier that frees tensor memory.
+    if (warp >= kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+        if (warp == kCopyWarp) {
+            // Q of both tiles, then K and V of each step: tile i of the sequence
+            // K 0, V 0, K 1, V 1, ... goes to stage i % kStages
+            if (lane == 0)
+                for (int x = 0; x < 2; ++x)
+                    if (n_step[x] > 0) {
+                        mbar_expect_tx(bQ + 8 * x, (uint32_t)(tile_tok * group * 128 * HALVES));
+                        for (int h = 0; h < HALVES; ++h)
+                            tma_load_3d(smem_u32(sQ + x * C::TILE_BYTES + h * C::HALF_BYTES), &map_q, bQ + 8 * x,
+                                        64 * h, kvh * group, (int)(t.tok0 + tok[x]));
+                    }
+            const int box = min(page_size, kTile);           // tokens of a copy
+            const int boxes = kTile / box;                   // copies of 64 dims of a tile
+            const int part = lane % boxes, half = lane / boxes;
+            bool ok = true;
+            uint32_t i = 0;
+            for (int j = 0; j < steps && ok; ++j) {
+                const int64_t key = k0 + (int64_t)j * kTile + part * box;
+                int page = -1, off = 0;
+                if (half < HALVES && key < k1 && key + box > lo) {
+                    const int col = (int)key / page_size;
+                    page = table[col];
+                    off = (int)key - col * page_size;
+                    if (page < 0 || page >= a.cache.n_pages) page = -1;
+                }
+                for (int v = 0; v < 2; ++v, ++i) {
+                    const uint32_t s = i % kStages;
+                    if (lane == 0) {
+                        if (i >= kStages) ok = mbar_wait(bEmpty + 8 * s, (i / kStages - 1) & 1, a.err, kErrPagedWait);
+                        if (ok) mbar_expect_tx(bFull + 8 * s, C::TILE_BYTES);
+                    }
+                    ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                    if (!ok) break;
+                    if (half < HALVES)
+                        tma_load_4d(smem_u32(sKV + s * C::TILE_BYTES + half * C::HALF_BYTES + part * box * 128),
+                                    v ? &map_v : &map_k, bFull + 8 * s, 64 * half, off, kvh, page);
+                }
+            }
+            // the last copy into each stage has landed (consumed already, unless
+            // a wait ran out)
+            if (lane == 0) {
+                for (uint32_t c = i > kStages ? i - kStages : 0; c < i; ++c)
+                    mbar_wait(bFull + 8 * (c % kStages), (c / kStages) & 1, a.err, kErrPagedWait, TC_DRAIN_NS);
+                for (int x = 0; x < 2; ++x)
+                    if (n_step[x] > 0) mbar_wait(bQ + 8 * x, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
+            }
+            __syncwarp();
+        } else if (warp == kMmaWarp) {
+            const uint32_t id_s = idesc_of(BF16, 0, kTile), id_o = idesc_of(BF16, 1, DP);
+            bool ok = true;
+            auto full = [&](uint32_t i) {  // tile i of the copy sequence has landed
+                if (ok) ok = mbar_wait(bFull + 8 * (i % kStages), (i / kStages) & 1, a.err, kErrPagedWait);
+                ok = __all_sync(0xffffffffu, ok);
+            };
+            auto score = [&](int x, int j) {  // S[x] = Q[x] K_j^T
+                if (lane == 0) {
+                    fence_after_sync();
+                    const uint32_t q = smem_u32(sQ + x * C::TILE_BYTES),
+                                   k = smem_u32(sKV + (2 * j) % kStages * C::TILE_BYTES);
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d) {
+                        const uint32_t at = d / 4 * C::HALF_BYTES + d % 4 * 32;
+                        mma_f16(tmem + C::S0 + x * kTile, sdesc128(q + at, 16, 1024), sdesc128(k + at, 16, 1024), id_s,
+                                d > 0);
+                    }
+                    mma_commit(bS + 8 * x);
+                }
+                __syncwarp();
+            };
+            for (int x = 0; x < 2; ++x)
+                if (n_step[x] > 0) {
+                    if (ok) ok = mbar_wait(bQ + 8 * x, 0, a.err, kErrPagedWait);
+                    full(0);
+                    if (ok) score(x, 0);
+                }
+            if (steps > 0 && ok && lane == 0) mma_commit(bEmpty);
+            for (int j = 0; j < steps && ok; ++j) {
+                const uint32_t iv = 2 * j + 1, ik = 2 * j + 2;  // V_j and K_{j + 1} in the copy sequence
+                full(iv);
+                if (!ok) break;
+                // the rows of V outside the block's keys become 0
+                const int64_t key0 = k0 + (int64_t)j * kTile;
+                const int r_lo = (int)max(min(lo - key0, (int64_t)kTile), (int64_t)0);
+                const int r_hi = (int)min(k1 - key0, (int64_t)kTile);
+                uint8_t *sv = sKV + iv % kStages * C::TILE_BYTES;
+                if (r_lo > 0 || r_hi < kTile) {
+                    for (int e = lane; e < kTile * HALVES * 8; e += 32) {
+                        const int row = (e >> 3) % kTile, h = e / (kTile * 8);
+                        if (row < r_lo || row >= r_hi)
+                            *reinterpret_cast<uint4 *>(sv + h * C::HALF_BYTES + row * 128 + (e & 7) * 16) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                for (int x = 0; x < 2 && ok; ++x) {
+                    if (j >= n_step[x]) continue;
+                    ok = mbar_wait(bP + 8 * x, j & 1, a.err, kErrPagedWait);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        fence_after_sync();
+                        const uint32_t v = smem_u32(sv);
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; ++k)
+                            mma_f16_ts(tmem + C::O0 + x * DP, tmem + C::P0 + x * C::P_STEP + k * 8,
+                                       sdesc128(v + k * 2048, C::HALF_BYTES, 1024), id_o, j > 0 || k > 0);
+                        mma_commit(bPV + 8 * x);
+                    }
+                    __syncwarp();
+                    if (j + 1 < n_step[x]) {
+                        full(ik);
+                        if (C::P_OVER_S && ok) {
+                            ok = mbar_wait(bPV + 8 * x, j & 1, a.err, kErrPagedWait);
+                            ok = __all_sync(0xffffffffu, ok);
+                        }
+                        if (ok) score(x, j + 1);
+                    }
+                }
+                if (ok && lane == 0) {
+                    mma_commit(bEmpty + 8 * (iv % kStages));
+                    if (j + 1 < steps) mma_commit(bEmpty + 8 * (ik % kStages));
+                }
+            }
+            // every MMA issued has completed before tensor memory is freed
+            if (lane == 0) {
+                mma_commit(bDrain);
+                mbar_wait(bDrain, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
+            }
+            __syncwarp();
+        }
+        asm volatile("bar.sync 0;" ::: "memory");
+        if (warp == kMmaWarp) {
+            fence_after_sync();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
+        const int x = warp >> 2, row = tid & (kTile - 1);
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
+        const uint32_t tS = tmem + C::S0 + x * kTile + lanes, tO = tmem + C::O0 + x * DP + lanes,
+                       tP = tmem + C::P0 + x * C::P_STEP + lanes;
+        const int i = row / group;
+        const bool live = i < n_tok[x] && row < tile_tok * group;
+        const int64_t tq = t.tok0 + tok[x] + i;
+        const int head = kvh * group + row % group;
+        // the keys this row sees, [see_lo, see_hi)
+        const int64_t pos = (int64_t)t.base + tok[x] + i;
+        const int64_t see_hi = live ? min(min(pos + 1, cap), k1) : 0;
+        const int64_t see_lo = a.window > 0 ? pos - a.window + 1 : 0;
+        // scores in base 2; a negative scale is the positive one of -S, and a
+        // scale of 0 a tiny one (masked scores are -inf, and 0 inf is a NaN)
+        const float sc = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
+        const bool flip = a.scale < 0.f;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        const int n = n_step[x];
+        for (int j = 0; j < n && ok; ++j) {
+            const int64_t key0 = k0 + (int64_t)j * kTile;
+            // pages of this step that are missing, a bit each
+            const int shift = 31 - __clz(min(page_size, kTile)), boxes = kTile >> shift;
+            bool gone = false;
+            {
+                const int64_t key = key0 + ((int64_t)lane << shift);
+                if (lane < boxes && key < k1) {
+                    const int page = table[(int)key / page_size];
+                    gone = page < 0 || page >= a.cache.n_pages;
+                }
+            }
+            const uint32_t missing = __ballot_sync(0xffffffffu, gone);
+            ok = mbar_wait(bS + 8 * x, j & 1, a.err, kErrPagedWait);
+            // the product of the step before is complete too (P_OVER_S: the
+            // issuer waited for it); its barrier's phases are taken in turn
+            if (!C::P_OVER_S && j > 0 && ok) ok = mbar_wait(bPV + 8 * x, (j - 1) & 1, a.err, kErrPagedWait);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after_sync();
+            float s[kTile];
+#pragma unroll
+            for (int c = 0; c < kTile; c += 32) tmem_get32(tS + c, s + c);
+            tmem_get_wait();
+            if (flip) {
+#pragma unroll
+                for (int c = 0; c < kTile; ++c) s[c] = -s[c];
+            }
+            // masked scores
+            if (key0 < see_lo || key0 + kTile > see_hi || missing) {
+                const int c0 = (int)max(min(see_lo - key0, (int64_t)kTile), (int64_t)0),
+                          c1 = (int)max(min(see_hi - key0, (int64_t)kTile), (int64_t)0);
+#pragma unroll
+                for (int c = 0; c < kTile; ++c)
+                    if (c < c0 || c >= c1) s[c] = -INFINITY;
+                if (missing) {
+#pragma unroll
+                    for (int c = 0; c < kTile; ++c)
+                        if (missing >> (c >> shift) & 1) s[c] = -INFINITY;
+                }
+            }
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
+            const float m_new = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
+            if (j == 0) {
+                m = m_new;
+            } else if (__any_sync(0xffffffffu, (m_new - m) * sc > kGrow)) {
+                // O of the steps before is complete: the commit behind this
+                // step's S covers their products too
+                const float f = m_new == m ? 1.f : pow2((m - m_new) * sc);
+                m = m_new;
+                l *= f;
+#pragma unroll
+                for (int c = 0; c < DP; c += 32) {
+                    float o[32];
+                    tmem_get32(tO + c, o);
+                    tmem_get_wait();
+                    uint32_t u[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * f);
+                    tmem_put32(tO + c, u);
+                }
+            }
+            const float ref = m == -INFINITY ? 0.f : -m * sc;
+            const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
+            float2 add = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < kTile; c += 64) {
+                uint32_t u[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const float2 y = f2fma(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), sc2, ref2);
+                    const float2 p = make_float2(pow2(y.x), pow2(y.y));
+                    add = f2add(add, p);
+                    u[e] = pack2(p.x, p.y, T());
+                }
+                tmem_put32(tP + c / 2, u);
+            }
+            l += add.x + add.y;
+            tmem_put_wait();
+            fence_before_sync();
+            mbar_arrive(bP + 8 * x);
+        }
+        if (n > 0 && ok) ok = mbar_wait(bPV + 8 * x, (n - 1) & 1, a.err, kErrPagedWait);
+        ok = __all_sync(0xffffffffu, ok);
+        fence_after_sync();
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a NaN sum stays one
+        const int64_t part = (tq * a.n_heads + head) * a.splits + sp;
+        if (n_pieces > 1 && live && ok) a.part_ml[part] = make_float2(n > 0 ? m * sc : -INFINITY, l);
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            if (n > 0 && ok) {
+                tmem_get32(tO + c, o);
+                tmem_get_wait();
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.f;
+            }
+            if (!live || !ok) continue;
+            if (n_pieces > 1) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    if (c + e < D)
+                        *reinterpret_cast<float4 *>(a.part_o + part * D + c + e) =
+                            make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            } else {
+                T *out = (T *)a.out + tq * a.out_stride + (int64_t)head * D + c;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+                    if (c + e < D)
+                        *reinterpret_cast<uint4 *>(out + e) =
+                            make_uint4(pack2(o[e] * inv, o[e + 1] * inv, T()),
+                                       pack2(o[e + 2] * inv, o[e + 3] * inv, T()),
+                                       pack2(o[e + 4] * inv, o[e + 5] * inv, T()),
+                                       pack2(o[e + 6] * inv, o[e + 7] * inv, T()));
+            }
+        }
+        fence_before_sync();
+        if (n_pieces > 1) __threadfence();
+        asm volatile("bar.sync 0;" ::: "memory");
+        if (n_pieces == 1) return;
+
+        // join the pieces: the block that arrives last, a warp per row
+        unsigned *count = a.count + (int64_t)blockIdx.x * gridDim.y + kvh;
+        if (tid == 0) last_s = atomicAdd(count, 1u) == (unsigned)n_pieces - 1;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (!last_s) return;
+        __threadfence();
+        if (tid == 0) *count = 0;
+        const int rows = (n_tok[0] + n_tok[1]) * group;
+        for (int row = warp; row < rows; row += kMmaWarp) {
+            const int64_t tq = t.tok0 + tok_first + row / group;
+            const int head = kvh * group + row % group;
+            const int64_t part = (tq * a.n_heads + head) * a.splits;
+            float top = -INFINITY;
+            for (int s = 0; s < n_pieces; ++s) top = fmaxf(top, __ldcg(&a.part_ml[part + s]).x);
+            const float ref = top == -INFINITY ? 0.f : top;
+            float l = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < n_pieces; ++s) {
+                const float2 ml = __ldcg(&a.part_ml[part + s]);
+                const float f = exp2f(ml.x - ref);
+                l += f * ml.y;
+                if (lane * 4 < D) {
+                    const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part_o + (part + s) * D) + lane);
+                    acc.x += f * o.x, acc.y += f * o.y, acc.z += f * o.z, acc.w += f * o.w;
+                }
+            }
+            const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+            if (lane * 4 < D)
+                *reinterpret_cast<uint2 *>((T *)a.out + tq * a.out_stride + (int64_t)head * D + lane * 4) =
+                    make_uint2(pack2(acc.x * inv, acc.y * inv, T()), pack2(acc.z * inv, acc.w * inv, T()));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> g_encode{nullptr};
+
+static cudaError_t encoder(PFN_cuTensorMapEncodeTiled_v12000 *out) {
+    *out = g_encode.load(std::memory_order_acquire);
+    if (*out) return cudaSuccess;
+    cudaDriverEntryPointQueryResult q;
+    void *fn = nullptr;
+    cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q);
+    if (e != cudaSuccess) return e;
+    if (q != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
+    *out = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+    g_encode.store(*out, std::memory_order_release);
+    return cudaSuccess;
+}
+
+// Swizzled tiles are made of blocks of 8 rows: a step's 128 keys are whole
+// pages of 8, 16, 32, 64 or 128 tokens, or lie in one page of a multiple of
+// 128. Tensor-map strides are below 2^40 bytes and not 0.
+bool paged_chunk_serves(const PagedCacheView &c, int n_heads) {
+    const bool page = c.page_size >= 8 && (kTile % c.page_size == 0 || c.page_size % kTile == 0);
+    const int64_t most = (int64_t)1 << 39;
+    return page && n_heads / c.n_kv_heads <= kTile && c.token_stride > 0 && c.token_stride < most &&
+           c.head_stride > 0 && c.head_stride < most && c.page_stride > 0 && c.page_stride < most;
+}
+
+int paged_chunk_unit(int group) { return 2 * (kTile / group) * group; }
+
+static bool cache_map(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap *m, const PagedCacheView &c,
+                      const void *base) {
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv_heads,
+                                (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.token_stride * 2, (cuuint64_t)c.head_stride * 2,
+                                   (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(c.page_size < kTile ? c.page_size : kTile), 1, 1};
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    return encode(m, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void *)base, dims,
+                  strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP>
+static cudaError_t launch_chunk(const PagedAttnArgs &a, int64_t tiles, const CUtensorMap &q, const CUtensorMap &k,
+                                const CUtensorMap &v, cudaStream_t st) {
+    static std::atomic<bool> attr[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!attr[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(k_paged_attn_chunk<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 ChunkCfg<DP>::SMEM);
+        if (e != cudaSuccess) return e;
+        attr[dev].store(true, std::memory_order_release);
+    }
+    const dim3 grid((unsigned)tiles, (unsigned)a.cache.n_kv_heads, (unsigned)a.splits);
+    k_paged_attn_chunk<T, DP><<<grid, kThreads, ChunkCfg<DP>::SMEM, st>>>(a, q, k, v);
+    return cudaGetLastError();
+}
+
+cudaError_t paged_chunk_attn(const PagedAttnArgs &a, cudaStream_t st) {
+    const PagedCacheView &c = a.cache;
+    const int group = a.n_heads / c.n_kv_heads, tile_tok = kTile / group;
+    PFN_cuTensorMapEncodeTiled_v12000 encode;
+    cudaError_t e = encoder(&encode);
+    if (e != cudaSuccess) return e;
+    CUtensorMap mq, mk, mv;
+    const cuuint64_t dims[3] = {(cuuint64_t)c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)tile_tok};
+    const cuuint32_t step[3] = {1, 1, 1};
+    if (encode(&mq, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void *)a.q, dims,
+               strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+        !cache_map(encode, &mk, c, c.k) || !cache_map(encode, &mv, c, c.v))
+        return cudaErrorInvalidValue;
+    const int64_t tiles = a.n_tokens / (2 * tile_tok) + a.n_seqs;
+    if (c.head_dim <= 64)
+        return c.bf16 ? launch_chunk<__nv_bfloat16, 64>(a, tiles, mq, mk, mv, st)
+                      : launch_chunk<__half, 64>(a, tiles, mq, mk, mv, st);
+    return c.bf16 ? launch_chunk<__nv_bfloat16, 128>(a, tiles, mq, mk, mv, st)
+                  : launch_chunk<__half, 128>(a, tiles, mq, mk, mv, st);
+}
+
+}  // namespace kk

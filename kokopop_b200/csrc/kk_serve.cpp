@@ -69,7 +69,8 @@ int kk_page_tables_device(kk_ctx *ctx, int32_t n_seqs, int32_t page_size, int32_
         need(ctx && ctx_len && new_len && free_range && table && seq_len && cu_new && status, "null argument");
         need(n_seqs >= 1 && page_size >= 1 && max_pages >= 1, "n_seqs, page_size or max_pages below 1");
         need(n_free >= 0 && (free_pages || n_free == 0), "null free_pages or negative n_free");
-        need(n_tokens >= 0 && n_tokens <= kMaxTokens && (slots || n_tokens == 0), "null slots or n_tokens out of range");
+        need(n_tokens >= 0 && n_tokens <= kMaxTokens, "n_tokens out of range");
+        need(slots || n_tokens == 0, "null slots");
         need((uintptr_t)(free_range + 2) <= (uintptr_t)status || (uintptr_t)(status + 3) <= (uintptr_t)free_range,
              "status overlaps free_range");
         use_device(ctx);
@@ -147,8 +148,9 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         need(q_stride >= row && out_stride >= row && q_stride % 8 == 0 && out_stride % 8 == 0,
              "q and out strides must hold a row and be multiples of 8 values");
         const int group = n_heads / a.cache.n_kv_heads;
-        const int64_t tiles = paged_attn_tiles(n_tokens, n_seqs, group);
-        need(tiles <= INT32_MAX && n_tokens * group <= INT32_MAX, "n_tokens x query heads per key head out of range");
+        const PagedAttnPlan plan = paged_attn_plan(a.cache, n_heads, n_tokens, n_seqs, max_new);
+        need(plan.tiles <= INT32_MAX && n_tokens * group <= INT32_MAX,
+             "n_tokens x query heads per key head out of range");
         use_device(ctx);
         cudaStream_t st = stream_of(ctx, stream);
         a.n_seqs = n_seqs;
@@ -167,17 +169,20 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         a.part_o = nullptr;
         a.part_ml = nullptr;
         a.count = nullptr;
-        // pieces of the key axis: enough blocks for about four rounds of two
-        // blocks on each of 148 SMs, 128 keys or more each
-        const int64_t most_rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
-        const int64_t blocks = std::min(tiles, n_seqs * ((most_rows + 15) / 16)) * a.cache.n_kv_heads;
+        a.err = (int *)ctx->d_err.p;
+        // pieces of the key axis: enough blocks for about four rounds of the
+        // row kernel's two blocks on each of 148 SMs (the chunk kernel: two
+        // rounds of its one), 128 keys or more each
+        const int64_t rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
+        const int64_t blocks = std::min(plan.tiles, n_seqs * ((rows + plan.unit - 1) / plan.unit)) * a.cache.n_kv_heads;
         int64_t keys = std::max(max_len, 1);
-        if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + 16);
-        const int64_t splits = std::min((1184 + blocks - 1) / blocks, (keys + 127) / 128);
+        if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + plan.unit / group + 16);
+        const int64_t want = plan.chunk ? 296 : 1184, step = plan.chunk ? 128 : 64;
+        const int64_t splits = std::min((want + blocks - 1) / blocks, (keys + 127) / 128);
         a.splits = capturing(st) ? 1 : (int)std::min<int64_t>(splits, 256);
-        a.split_keys = (int)(((keys + a.splits - 1) / a.splits + 63) / 64 * 64);
+        a.split_keys = (int)(((keys + a.splits - 1) / a.splits + step - 1) / step * step);
         if (a.splits == 1) {
-            check_cuda(paged_attn(a, st), "paged attention launch");
+            check_cuda(paged_attn(plan, a, st), "paged attention launch");
             ++ctx->n_launches;
             return KK_OK;
         }
@@ -186,13 +191,13 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         a.part_o = ctx->buf("paged_part_o", parts * a.cache.head_dim);
         a.part_ml = (float2 *)ctx->buf("paged_part_ml", parts * 2);
         DevBuf &count = ctx->ws["paged_count"];
-        const size_t count_bytes = (size_t)tiles * a.cache.n_kv_heads * sizeof(unsigned);
+        const size_t count_bytes = (size_t)plan.tiles * a.cache.n_kv_heads * sizeof(unsigned);
         if (count.bytes < count_bytes) {
             count.ensure(count_bytes);
             check_cuda(cudaMemsetAsync(count.p, 0, count.bytes, st), "clear the piece counters");
         }
         a.count = (unsigned *)count.p;
-        check_cuda(paged_attn(a, st), "paged attention launch");
+        check_cuda(paged_attn(plan, a, st), "paged attention launch");
         ++ctx->n_launches;
         return KK_OK;
     });
