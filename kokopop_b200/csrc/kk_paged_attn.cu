@@ -14,38 +14,48 @@
 //
 // k_paged_attn_row: for one or a few queries per key head, bytes bound it:
 // every key and value of the request is read once for the `group` heads that
-// share it. A block takes 16 rows (query, head of the group) of one key head
-// as the M = 16 side of mma.sync.m16n8k16, so that a single token of a group
-// of up to 16 heads reads its keys once; one piece of the key axis per block
-// keeps all SMs reading when there are few rows. Each of the 4 warps walks its
-// own blocks of 16 keys with its own ring of asynchronous 16-byte copies (no
-// block barrier in the loop) and its own running maximum and sum; the warps
-// are joined in shared memory, the pieces in global memory by the block that
-// arrives last, in the order of the pieces, so that the result does not
-// depend on which one that is.
+// share it. A block takes 8 or 16 rows (query, head of the group) of one key
+// head and one piece of the key axis; each of its 4 warps walks blocks of 16
+// keys of its own, with its own ring of copies in flight (no block barrier in
+// the loop) and its own running maximum and sum. The products are transposed,
+// S^T = K Q^T and O^T = V^T P^T, so that the 16 keys (or 16 dims) are the M
+// side of mma.sync.m16n8k16 and the few rows its N side: nothing is computed
+// for rows that do not exist beyond the next multiple of 8. The maximum is
+// followed lazily as in kk_paged_chunk.cu, so most steps exchange nothing
+// between lanes but one vote. Pages whose size is 8 or a multiple of 16 come
+// by tensor copies (one lane issues a block's copy of 64 dims), others by
+// 16-byte asynchronous copies. The warps are joined in shared memory, the
+// pieces in global memory by the block that arrives last, in the order of the
+// pieces, so that the result does not depend on which one that is.
 #include "kk_paged_attn.cuh"
+#include "kk_ptx.cuh"
+
+#include <cuda.h>
 
 #include <atomic>
+#include <cstring>
 
 namespace kk {
 
 namespace {
 
-constexpr int kRows = 16;   // query rows of a block
 constexpr int kKeys = 16;   // keys of a warp's step
 constexpr int kWarps = 4;
 constexpr int kStages = 3;
+constexpr int kFewRows = 16;  // query rows up to which a call takes this kernel
+constexpr int kMaxPieces = 256;
+constexpr float kGrow = 8.0f;  // base-2 growth of a maximum that is left alone
 
-template <int DP>
+template <int DP, int NB>
 struct RowCfg {
-    static constexpr int ROW_BYTES = DP * 2;
-    static constexpr int TILE = kKeys * ROW_BYTES;  // K or V of one step
+    static constexpr int ROWS = 8 * NB;
+    static constexpr int HALF_BYTES = kKeys * 128;   // 64 dims of a block of keys
+    static constexpr int TILE = kKeys * DP * 2;      // K or V of one step
     static constexpr int RING = kWarps * kStages * 2 * TILE;
-    static constexpr int JOIN = kWarps * kRows * (DP + 2) * 4;
-    static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+    static constexpr int OS = DP + 4;                // row stride of the join: no bank twice
+    static constexpr int JOIN = (kWarps * ROWS * (OS + 2) + ROWS * (kMaxPieces + 1)) * 4;
+    static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + 1024 /*align*/;
 };
-
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // 16 bytes of global memory, or zeros (live 0; src is then not read)
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
@@ -88,267 +98,405 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// An 8 x 8 matrix of 16-bit values over the lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+// 4 values of an output row, divided by the sum of its weights
+template <typename T>
+__device__ __forceinline__ void put_row4(T *out, float4 v, float l) {
+    const float inv = paged_inverse(l);
+    *reinterpret_cast<uint2 *>(out) =
+        make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
+}
+
 }  // namespace
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kWarps * 32) k_paged_attn_row(PagedAttnArgs a) {
-    using C = RowCfg<DP>;
-    constexpr int KC = DP / 16;      // k-steps of a score
-    constexpr int NT = DP / 8;       // n-tiles of an output row
+template <typename T, int DP, int NB, bool TMA>
+__global__ void __launch_bounds__(kWarps * 32)
+    k_paged_attn_row(PagedAttnArgs a, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v) {
+    using C = RowCfg<DP, NB>;
+    constexpr int KC = DP / 16;      // k-steps of a score, m-tiles of an output
+    constexpr int HALVES = DP / 64;
     constexpr int CH = DP / 8;       // 16-byte chunks of a key
-    extern __shared__ __align__(128) unsigned char sm[];
+    extern __shared__ __align__(1024) unsigned char sm_raw[];
+    unsigned char *sm = (unsigned char *)(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t bar_s[kWarps][kStages];
     __shared__ uint32_t seen_s[kWarps][kStages];
     __shared__ unsigned last_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
     const int group = a.n_heads / a.cache.n_kv_heads, kvh = blockIdx.y;
-    const RowTile t = find_tile(a, group, kRows, blockIdx.x);
+    const RowTile t = find_tile(a, group, C::ROWS, blockIdx.x);
     if (t.r < 0) return;  // the whole block
-    const int D = a.cache.head_dim;
+    const int D = a.cache.head_dim, page_size = a.cache.page_size;
 
-    // the rows' positions and key ranges; the block's range
-    const int base = t.base;
-    const int rows_here = min(kRows, t.rows - t.row0);
-    const int pos_first = base + t.row0 / group, pos_last = base + (t.row0 + rows_here - 1) / group;
-    int64_t kend = min((int64_t)pos_last + 1, (int64_t)a.max_pages * a.cache.page_size);
-    int64_t kbeg = a.window > 0 ? max((int64_t)pos_first - a.window + 1, (int64_t)0) : 0;
-    kbeg = kbeg / kKeys * kKeys;
-    if (kend < kbeg) kend = kbeg;
-    // pieces: at least split_keys keys each, so that splits of them reach the end
+    // the rows' positions and key ranges; the block's range and piece
+    const int rows_here = min(C::ROWS, t.rows - t.row0);
+    const int pos_first = t.base + t.row0 / group, pos_last = t.base + (t.row0 + rows_here - 1) / group;
+    const int64_t cap = (int64_t)a.max_pages * page_size;
+    const int64_t lo = a.window > 0 ? max((int64_t)pos_first - a.window + 1, (int64_t)0) : 0;
+    const int64_t kbeg = lo / kKeys * kKeys, kend = max(min((int64_t)pos_last + 1, cap), kbeg);
     int64_t piece = (kend - kbeg + a.splits - 1) / a.splits;
     piece = max((piece + 63) / 64 * 64, (int64_t)a.split_keys);
     const int n_pieces = (int)max((kend - kbeg + piece - 1) / piece, (int64_t)1);
     const int sp = blockIdx.z;
     if (sp >= n_pieces) return;
-    const int64_t k0 = kbeg + sp * piece, k1 = min(k0 + piece, kend);
-
-    // Q fragments: rows gid and gid + 8
-    uint32_t qf[KC][4];
-    int lim_hi[2], lim_lo[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = t.row0 + gid + 8 * i;
-        const bool live = gid + 8 * i < rows_here;
-        const int tok = row / group, head = kvh * group + row % group;
-        lim_hi[i] = live ? base + tok : -1;
-        lim_lo[i] = live && a.window > 0 ? base + tok - a.window + 1 : 0;
-        const T *q = (const T *)a.q + (t.tok0 + tok) * a.q_stride + (int64_t)head * D;
-#pragma unroll
-        for (int k = 0; k < KC; ++k) {
-            const int d = k * 16 + tig * 2;
-            qf[k][i] = live && d < D ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
-            qf[k][2 + i] = live && d + 8 < D ? *reinterpret_cast<const uint32_t *>(q + d + 8) : 0u;
-        }
-    }
-
-    float o[NT][4];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    // keys are below 2^31: positions are 32-bit
+    const int k0 = (int)(kbeg + sp * piece), k1 = (int)min((int64_t)k0 + piece, kend);
 
     // this warp's steps: blocks of kKeys keys, kWarps apart
-    const int n_blocks = (int)((k1 - k0 + kKeys - 1) / kKeys);
+    const int n_blocks = (k1 - k0 + kKeys - 1) / kKeys;
     const int n_steps = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;
     unsigned char *ring = sm + warp * kStages * 2 * C::TILE;
+    const uint32_t ring_u = smem_u32(ring), bars = smem_u32(bar_s[warp]);
     const T *kc = (const T *)a.cache.k + kvh * a.cache.head_stride;
     const T *vc = (const T *)a.cache.v + kvh * a.cache.head_stride;
     const int32_t *table = a.table + (int64_t)t.r * a.max_pages;
+    if (TMA) {
+        if (lane == 0) {
+            for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+    }
 
+    const int box = min(page_size, kKeys), boxes = kKeys / box;  // TMA: tokens of a copy, copies of a block
     auto issue = [&](int s) {
         if (s < n_steps) {
-            const int64_t key0 = k0 + (int64_t)(warp + s * kWarps) * kKeys;
-            // lane = key: where its row lies
-            int64_t at = -1;
-            const int64_t key = key0 + (lane & (kKeys - 1));
-            if (key < k1) {
-                const int64_t col = key / a.cache.page_size;
-                const int page = table[col];
-                if (page >= 0 && page < a.cache.n_pages)
-                    at = page * a.cache.page_stride + (key - col * a.cache.page_size) * a.cache.token_stride;
-            }
-            const uint32_t seen = __ballot_sync(0xffffffffu, at >= 0) & ((1u << kKeys) - 1);
-            unsigned char *kt = ring + (s % kStages) * 2 * C::TILE;
-            if (lane == 0) seen_s[warp][s % kStages] = seen;
+            const int key0 = k0 + (warp + s * kWarps) * kKeys, st = s % kStages;
+            if (TMA) {
+                const int part = lane & (boxes - 1), half = (lane / boxes) % HALVES, v = lane / (boxes * HALVES);
+                const int key = key0 + part * box;
+                int page = -1, off = 0;
+                if (v < 2 && key < k1) {
+                    const int col = key / page_size;
+                    page = table[col];
+                    off = key - col * page_size;
+                    if (page < 0 || page >= a.cache.n_pages) page = -1;
+                }
+                const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
+                if (lane == 0) {
+                    seen_s[warp][st] = boxes == 1 ? (have & 1 ? 0xffffu : 0u)
+                                                  : (have & 1 ? 0xffu : 0u) | (have & 2 ? 0xff00u : 0u);
+                    mbar_expect_tx(bars + 8 * st, 2 * C::TILE);
+                }
+                __syncwarp();
+                if (v < 2)
+                    tma_load_4d(ring_u + (st * 2 + v) * C::TILE + half * C::HALF_BYTES + part * box * 128,
+                                v ? &map_v : &map_k, bars + 8 * st, 64 * half, off, kvh, page);
+            } else {
+                // lane = key: where its row lies
+                int64_t at = -1;
+                const int key = key0 + (lane & (kKeys - 1));
+                if (key < k1 && key >= lo) {
+                    const int col = key / page_size, page = table[col];
+                    if (page >= 0 && page < a.cache.n_pages)
+                        at = page * a.cache.page_stride + (key - col * page_size) * a.cache.token_stride;
+                }
+                const uint32_t seen = __ballot_sync(0xffffffffu, at >= 0) & ((1u << kKeys) - 1);
+                if (lane == 0) seen_s[warp][st] = seen;
 #pragma unroll
-            for (int i = lane; i < kKeys * CH; i += 32) {
-                const int row = i / CH, ch = i % CH;
-                const int64_t off = __shfl_sync(0xffffffffu, at, row);
-                const bool live = off >= 0 && ch * 8 < D;
-                const int64_t e = live ? off + ch * 8 : 0;
-                const uint32_t dst = smem_addr(kt) + row * C::ROW_BYTES + ((ch ^ (row & 7)) * 16);
-                cp16(dst, kc + e, live);
-                cp16(dst + C::TILE, vc + e, live);
+                for (int i = lane; i < kKeys * CH; i += 32) {
+                    const int row = i / CH, ch = i % CH;
+                    const int64_t off = __shfl_sync(0xffffffffu, at, row);
+                    const bool live = off >= 0 && ch * 8 < D;
+                    const int64_t e = live ? off + ch * 8 : 0;
+                    const uint32_t dst = ring_u + st * 2 * C::TILE + (ch >> 3) * C::HALF_BYTES + row * 128 +
+                                         (((ch ^ row) & 7) * 16);
+                    cp16(dst, kc + e, live);
+                    cp16(dst + C::TILE, vc + e, live);
+                }
             }
         }
-        cp_commit();
+        if (!TMA) cp_commit();
     };
-
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) issue(s);
-    const float scale2 = a.scale * 1.4426950408889634f;  // scores in base 2
-    for (int s = 0; s < n_steps; ++s) {
-        issue(s + kStages - 1);
-        cp_wait<kStages - 1>();
-        __syncwarp();
-        const uint32_t kt = smem_addr(ring + (s % kStages) * 2 * C::TILE), vt = kt + C::TILE;
-        const uint32_t seen = seen_s[warp][s % kStages];
-        const int64_t key0 = k0 + (int64_t)(warp + s * kWarps) * kKeys;
-        float sc[2][4];
+
+    // Q^T fragments: columns (rows of Q) gid and, NB 2, gid + 8
+    uint32_t qf[KC][NB][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
+    for (int b = 0; b < NB; ++b) {
+        const int row = t.row0 + gid + 8 * b;
+        const bool live = gid + 8 * b < rows_here;
+        const T *q = (const T *)a.q + (t.tok0 + row / group) * a.q_stride + (int64_t)(kvh * group + row % group) * D;
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
-            // 16 keys x 16 dims: matrices (keys 0-7, d 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-            const int row = (lane & 7) + ((lane >> 4) << 3), ch = 2 * k + ((lane >> 3) & 1);
-            uint32_t b[4];
-            ldsm4(kt + row * C::ROW_BYTES + ((ch ^ (row & 7)) * 16), b);
-            mma16<T>(sc[0], qf[k], b[0], b[1]);
-            mma16<T>(sc[1], qf[k], b[2], b[3]);
+            const int d = k * 16 + tig * 2;
+            qf[k][b][0] = live && d < D ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
+            qf[k][b][1] = live && d + 8 < D ? *reinterpret_cast<const uint32_t *>(q + d + 8) : 0u;
         }
-        float top[2] = {-INFINITY, -INFINITY};
+    }
+    // the keys that this lane's columns (rows of Q 2 tig, 2 tig + 1) see
+    int see_hi[NB][2], see_lo[NB][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int col = i * 8 + tig * 2 + (e & 1), h = e >> 1;
-                const int64_t key = key0 + col;
-                const bool live = (seen >> col & 1) && key <= lim_hi[h] && key >= lim_lo[h];
-                sc[i][e] = live ? sc[i][e] * scale2 : -INFINITY;
-                top[h] = fmaxf(top[h], sc[i][e]);
+        for (int e = 0; e < 2; ++e) {
+            const int i = 8 * b + 2 * tig + e, pos = t.base + (t.row0 + i) / group;
+            see_hi[b][e] = i < rows_here ? pos : -1;
+            see_lo[b][e] = i < rows_here && a.window > 0 ? pos - a.window + 1 : 0;
+        }
+
+    float o[KC][NB][4], mx[NB][2], sum[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        mx[b][0] = mx[b][1] = -INFINITY;
+        sum[b][0] = sum[b][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) o[i][b][0] = o[i][b][1] = o[i][b][2] = o[i][b][3] = 0.f;
+    }
+    const float scale2 = a.scale * 1.4426950408889634f;  // scores in base 2
+    // keys that every row sees need no mask
+    const int all_lo = a.window > 0 ? pos_last - a.window + 1 : 0, all_hi = min(pos_first, k1 - 1);
+    // lane's part of the fragments: K rows (m) and V rows (k, transposed)
+    const int k_row = (lane & 7) + (lane & 8), k_ch = lane >> 4;
+    const int v_row = (lane & 7) + ((lane >> 4) << 3), v_ch = (lane >> 3) & 1;
+    bool ok = true;
+    int s = 0;
+    for (; s < n_steps; ++s) {
+        issue(s + kStages - 1);
+        const int st = s % kStages;
+        if (TMA) {
+            ok = mbar_wait_tight(bars + 8 * st, (s / kStages) & 1, a.err, kErrPagedWait);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+        } else {
+            cp_wait<kStages - 1>();
+            __syncwarp();
+        }
+        const uint32_t kt = ring_u + st * 2 * C::TILE, vt = kt + C::TILE;
+        const uint32_t seen = seen_s[warp][st];
+        const int key0 = k0 + (warp + s * kWarps) * kKeys;
+        if (TMA && (key0 < lo || key0 + kKeys > k1)) {
+            // values of tokens outside the range may be anything, and 0 times
+            // a NaN is one: their rows become 0
+            for (int i = lane; i < kKeys * CH; i += 32) {
+                const int row = i / CH, ch = i % CH;
+                if (key0 + row < lo || key0 + row >= k1)
+                    *reinterpret_cast<uint4 *>(ring + (st * 2 + 1) * C::TILE + (ch >> 3) * C::HALF_BYTES + row * 128 +
+                                               (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
-        uint32_t p[4];
-        float corr[2];
+            fence_proxy_async();  // before the next copy into this stage
+            __syncwarp();
+        }
+        float sc[NB][4], sd[NB][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-            const float m = fmaxf(mx[h], top[h]);
-            const float ref = m == -INFINITY ? 0.f : m;  // no key so far: every weight 0
-            corr[h] = exp2f(mx[h] - ref);
-            mx[h] = m;
-            float add = 0.f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float x = exp2f(sc[i][2 * h] - ref), y = exp2f(sc[i][2 * h + 1] - ref);
-                add += x + y;
-                p[2 * i + h] = pack2(x, y, T());
-            }
-            sum[h] = sum[h] * corr[h] + add;
+        for (int b = 0; b < NB; ++b) {
+            sc[b][0] = sc[b][1] = sc[b][2] = sc[b][3] = 0.f;
+            sd[b][0] = sd[b][1] = sd[b][2] = sd[b][3] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-            // 16 keys x 16 dims of V, transposed: (keys 0-7, d 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
-            const int row = (lane & 15), ch = 2 * j + (lane >> 4);
-            uint32_t b[4];
-            ldsm4t(vt + row * C::ROW_BYTES + ((ch ^ (row & 7)) * 16), b);
+        for (int k = 0; k < KC; k += 2) {  // two chains of products
+            uint32_t f[4], g[4];
+            ldsm4(kt + k / 4 * C::HALF_BYTES + k_row * 128 + ((((2 * k + k_ch) ^ k_row) & 7) * 16), f);
+            ldsm4(kt + k / 4 * C::HALF_BYTES + k_row * 128 + ((((2 * k + 2 + k_ch) ^ k_row) & 7) * 16), g);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float(&c)[4] = o[2 * j + i];
-                c[0] *= corr[0], c[1] *= corr[0], c[2] *= corr[1], c[3] *= corr[1];
-                mma16<T>(c, p, b[2 * i], b[2 * i + 1]);
+            for (int b = 0; b < NB; ++b) {
+                mma16<T>(sc[b], f, qf[k][b][0], qf[k][b][1]);
+                mma16<T>(sd[b], g, qf[k + 1][b][0], qf[k + 1][b][1]);
             }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[b][e] = (sc[b][e] + sd[b][e]) * scale2;
+        if (key0 < all_lo || key0 + kKeys - 1 > all_hi || seen != (1u << kKeys) - 1) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = gid + 8 * (e >> 1), key = key0 + i;
+                    if (!(seen >> i & 1) || key > see_hi[b][e & 1] || key < see_lo[b][e & 1] || key >= k1)
+                        sc[b][e] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(sc[b][e], sc[b][e + 2]) > mx[b][e] + kGrow;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float corr[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float m = fmaxf(fmaxf(sc[b][e], sc[b][e + 2]), mx[b][e]);
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    corr[e] = m == mx[b][e] ? 1.f : pow2(mx[b][e] - m);
+                    mx[b][e] = m;
+                    sum[b][e] *= corr[e];
+                }
+#pragma unroll
+                for (int i = 0; i < KC; ++i) {
+                    o[i][b][0] *= corr[0], o[i][b][1] *= corr[1];
+                    o[i][b][2] *= corr[0], o[i][b][3] *= corr[1];
+                }
+            }
+        }
+        uint32_t p[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float r0 = mx[b][0] == -INFINITY ? 0.f : mx[b][0], r1 = mx[b][1] == -INFINITY ? 0.f : mx[b][1];
+            const float x0 = pow2(sc[b][0] - r0), x1 = pow2(sc[b][1] - r1);
+            const float y0 = pow2(sc[b][2] - r0), y1 = pow2(sc[b][3] - r1);
+            sum[b][0] += x0 + y0;
+            sum[b][1] += x1 + y1;
+            // [key gid][row 2 tig, + 1] to [row gid][key 2 tig, + 1]
+            p[b][0] = transpose8(pack2(x0, x1, T()));
+            p[b][1] = transpose8(pack2(y0, y1, T()));
+        }
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            uint32_t f[4];
+            ldsm4t(vt + i / 4 * C::HALF_BYTES + v_row * 128 + ((((2 * i + v_ch) ^ v_row) & 7) * 16), f);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma16<T>(o[i][b], f, p[b][0], p[b][1]);
         }
         __syncwarp();  // the stage is read before its next copies are issued
     }
-    cp_wait<0>();
+    if (TMA) {
+        if (!ok)  // the copies still in flight land before the block ends
+            for (int c = s; c < min(s + kStages, n_steps); ++c)
+                mbar_wait(bars + 8 * (c % kStages), (c / kStages) & 1, a.err, kErrPagedWait, TC_DRAIN_NS);
+    } else {
+        cp_wait<0>();
+    }
     __syncthreads();
 
-    // join the warps: [warp][row][DP] values, then the maxima and sums
+    // join the warps: [warp][row][dim] values, then the maxima and sums
     float *jo = reinterpret_cast<float *>(sm);
-    float *jm = jo + kWarps * kRows * DP, *jl = jm + kWarps * kRows;
+    float *jm = jo + kWarps * C::ROWS * C::OS, *jl = jm + kWarps * C::ROWS, *jf = jl + kWarps * C::ROWS;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-        const int row = warp * kRows + gid + 8 * h;
-        if (tig == 0) jm[row] = mx[h], jl[row] = sum[h];
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-            *reinterpret_cast<float2 *>(jo + row * DP + j * 8 + tig * 2) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
-    }
-    __syncthreads();
-    constexpr int PER = kRows * DP / (kWarps * 32);  // values of a thread: PER of one row
-    const int row = tid * PER / DP, d0 = tid * PER % DP;
-    const bool live = row < rows_here;
-    const int g = t.row0 + row;
-    const int64_t tok = t.tok0 + g / group;
-    const int head = kvh * group + g % group;
-    float m = -INFINITY, l = 0.f, acc[PER];
+        for (int e = 0; e < 2; ++e) {
+            float l = sum[b][e];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const int row = warp * C::ROWS + 8 * b + 2 * tig + e;
+            if (gid == 0) jm[row] = mx[b][e], jl[row] = l;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, jm[w * kRows + row]);
-    const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(jm[w * kRows + row] - ref);
-        l += f * jl[w * kRows + row];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] += f * jo[(w * kRows + row) * DP + d0 + i];
-    }
-    if (n_pieces > 1) {
-        const int64_t part = (tok * a.n_heads + head) * a.splits;
-        if (live) {
-            for (int i = 0; i < PER; ++i)
-                if (d0 + i < D) a.part_o[(part + sp) * D + d0 + i] = acc[i];
-            if (d0 == 0) a.part_ml[part + sp] = make_float2(m, l);
-        }
-        __threadfence();
-        __syncthreads();
-        unsigned *count = a.count + (int64_t)blockIdx.x * gridDim.y + kvh;
-        if (tid == 0) last_s = atomicAdd(count, 1u) == (unsigned)n_pieces - 1;
-        __syncthreads();
-        if (!last_s) return;
-        __threadfence();
-        if (tid == 0) *count = 0;
-        m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-        if (live) {
-            for (int s = 0; s < n_pieces; ++s) m = fmaxf(m, __ldcg(&a.part_ml[part + s]).x);
-            const float all = m == -INFINITY ? 0.f : m;
-            for (int s = 0; s < n_pieces; ++s) {
-                const float2 ml = __ldcg(&a.part_ml[part + s]);
-                const float f = exp2f(ml.x - all);
-                l += f * ml.y;
-#pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (d0 + i < D) acc[i] += f * __ldcg(&a.part_o[(part + s) * D + d0 + i]);
+            for (int i = 0; i < KC; ++i) {
+                jo[row * C::OS + i * 16 + gid] = o[i][b][e];
+                jo[row * C::OS + i * 16 + gid + 8] = o[i][b][e + 2];
             }
         }
-    }
-    if (live) {
-        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a NaN sum stays one
-        T *out = (T *)a.out + tok * a.out_stride + (int64_t)head * D;
+    __syncthreads();
+    // a thread takes 4 dims of a row at a time
+    const int per_row = D / 4, items = rows_here * per_row;
+    for (int it = tid; it < items; it += kWarps * 32) {
+        const int row = it / per_row, d = (it - row * per_row) * 4, g = t.row0 + row;
+        const int64_t tok = t.tok0 + g / group;
+        const int head = kvh * group + g % group;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < PER; i += 2)
-            if (d0 + i < D) *reinterpret_cast<uint32_t *>(out + d0 + i) = pack2(acc[i] * inv, acc[i + 1] * inv, T());
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, jm[w * C::ROWS + row]);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = pow2(jm[w * C::ROWS + row] - ref);
+            l += f * jl[w * C::ROWS + row];
+            const float4 x = *reinterpret_cast<const float4 *>(jo + (w * C::ROWS + row) * C::OS + d);
+            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+        }
+        if (n_pieces > 1) {
+            const int64_t part = (tok * a.n_heads + head) * a.splits + sp;
+            *reinterpret_cast<float4 *>(a.part_o + part * D + d) = acc;
+            if (d == 0) a.part_ml[part] = make_float2(m, l);
+        } else {
+            put_row4((T *)a.out + tok * a.out_stride + (int64_t)head * D + d, acc, l);
+        }
+    }
+    if (n_pieces == 1) return;
+    __threadfence();
+    __syncthreads();
+    unsigned *count = a.count + (int64_t)blockIdx.x * gridDim.y + kvh;
+    if (tid == 0) last_s = atomicAdd(count, 1u) == (unsigned)n_pieces - 1;
+    __syncthreads();
+    if (!last_s) return;
+    __threadfence();
+    if (tid == 0) *count = 0;
+    // the factors of the pieces and the sum of each row, a warp per row
+    for (int row = warp; row < rows_here; row += kWarps) {
+        const int g = t.row0 + row;
+        const int64_t part = ((t.tok0 + g / group) * a.n_heads + kvh * group + g % group) * a.splits;
+        float m = -INFINITY, l = 0.f;
+        for (int i = lane; i < n_pieces; i += 32) m = fmaxf(m, __ldcg(&a.part_ml[part + i]).x);
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+        const float ref = m == -INFINITY ? 0.f : m;
+        for (int i = lane; i < n_pieces; i += 32) {
+            const float2 ml = __ldcg(&a.part_ml[part + i]);
+            const float f = pow2(ml.x - ref);
+            jf[row * (kMaxPieces + 1) + 1 + i] = f;
+            l += f * ml.y;
+        }
+        l = warp_sum(l);
+        if (lane == 0) jf[row * (kMaxPieces + 1)] = l;
+    }
+    __syncthreads();
+    for (int it = tid; it < items; it += kWarps * 32) {
+        const int row = it / per_row, d = (it - row * per_row) * 4, g = t.row0 + row;
+        const int64_t tok = t.tok0 + g / group;
+        const int head = kvh * group + g % group;
+        const float *f = jf + row * (kMaxPieces + 1) + 1;
+        const float *src = a.part_o + (tok * a.n_heads + head) * a.splits * D + d;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int i = 0; i < n_pieces; ++i) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(src + (int64_t)i * D));
+            acc.x += f[i] * x.x, acc.y += f[i] * x.y, acc.z += f[i] * x.z, acc.w += f[i] * x.w;
+        }
+        put_row4((T *)a.out + tok * a.out_stride + (int64_t)head * D + d, acc, f[-1]);
     }
 }
 
-template <typename T, int DP>
+// Block of kKeys keys in whole boxes of a page, strides a tensor map takes.
+static bool row_by_tensor(const PagedCacheView &c) {
+    return (c.page_size == 8 || c.page_size % kKeys == 0) && paged_strides_mappable(c);
+}
+
+template <typename T, int DP, int NB, bool TMA>
 static cudaError_t launch_row(const PagedAttnArgs &a, int64_t tiles, cudaStream_t st) {
     static std::atomic<bool> attr[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    using C = RowCfg<DP, NB>;
+    cudaError_t e = paged_smem_once(k_paged_attn_row<T, DP, NB, TMA>, C::SMEM, attr);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!attr[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(k_paged_attn_row<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 RowCfg<DP>::SMEM);
+    CUtensorMap mk, mv;
+    memset(&mk, 0, sizeof mk);
+    memset(&mv, 0, sizeof mv);
+    if (TMA) {
+        e = paged_cache_maps(a.cache, kKeys, &mk, &mv);
         if (e != cudaSuccess) return e;
-        attr[dev].store(true, std::memory_order_release);
     }
     const dim3 grid((unsigned)tiles, (unsigned)a.cache.n_kv_heads, (unsigned)a.splits);
-    k_paged_attn_row<T, DP><<<grid, kWarps * 32, RowCfg<DP>::SMEM, st>>>(a);
+    k_paged_attn_row<T, DP, NB, TMA><<<grid, kWarps * 32, C::SMEM, st>>>(a, mk, mv);
     return cudaGetLastError();
+}
+
+template <typename T, int DP>
+static cudaError_t launch_row_of(const PagedAttnPlan &p, const PagedAttnArgs &a, cudaStream_t st) {
+    const bool tma = row_by_tensor(a.cache);
+    if (p.unit == 8) return tma ? launch_row<T, DP, 1, true>(a, p.tiles, st) : launch_row<T, DP, 1, false>(a, p.tiles, st);
+    return tma ? launch_row<T, DP, 2, true>(a, p.tiles, st) : launch_row<T, DP, 2, false>(a, p.tiles, st);
 }
 
 PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new) {
     const int group = n_heads / c.n_kv_heads;
     const int64_t rows = (n_tokens < max_new ? n_tokens : max_new) * (int64_t)group;
     PagedAttnPlan p;
-    p.chunk = rows > kRows && paged_chunk_serves(c, n_heads);
-    p.unit = p.chunk ? paged_chunk_unit(group) : kRows;
+    p.chunk = rows > kFewRows && paged_chunk_serves(c, n_heads);
+    p.unit = p.chunk ? paged_chunk_unit(group) : rows > 8 ? 16 : 8;
     p.tiles = n_tokens * group / p.unit + n_seqs;
     return p;
 }
@@ -356,8 +504,8 @@ PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_to
 cudaError_t paged_attn(const PagedAttnPlan &p, const PagedAttnArgs &a, cudaStream_t st) {
     if (p.chunk) return paged_chunk_attn(a, st);
     if (a.cache.head_dim <= 64)
-        return a.cache.bf16 ? launch_row<__nv_bfloat16, 64>(a, p.tiles, st) : launch_row<__half, 64>(a, p.tiles, st);
-    return a.cache.bf16 ? launch_row<__nv_bfloat16, 128>(a, p.tiles, st) : launch_row<__half, 128>(a, p.tiles, st);
+        return a.cache.bf16 ? launch_row_of<__nv_bfloat16, 64>(p, a, st) : launch_row_of<__half, 64>(p, a, st);
+    return a.cache.bf16 ? launch_row_of<__nv_bfloat16, 128>(p, a, st) : launch_row_of<__half, 128>(p, a, st);
 }
 
 }  // namespace kk

@@ -1,9 +1,13 @@
-// What the two kernels of the paged attention share: the rounding of a pair
-// to the cache's type and the tile of a block.
+// What the two kernels of the paged attention share: arithmetic, the tile of
+// a block, and the tensor maps of the cache.
 #pragma once
 
 #include "kk_common.cuh"
 #include "kk_kernels.h"
+
+#include <cuda.h>
+
+#include <atomic>
 
 namespace kk {
 
@@ -16,10 +20,30 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// 2^x, results below 2^-126 as 0 (weights are at most 2^8 and rounded to 16
+// bits, or relative to a largest one)
+__device__ __forceinline__ float pow2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 1 / l; 0 for a row that saw no key, and a NaN sum stays one
+__device__ __forceinline__ float paged_inverse(float l) { return l > 0.f ? 1.f / l : l == 0.f ? 0.f : l; }
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z,
+                                            int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+
 // The tile `w` of a launch, `unit` rows (query, head of the group) each.
 // Request r's tiles begin at floor(cu[r] * group / unit) + r: consecutive
 // requests are at least as far apart as request r has tiles, so the request
-// is found by bisection of cu_new alone, and at most
+// is found from cu_new alone, and at most
 // floor(n_tokens * group / unit) + n_seqs indices are in use.
 struct RowTile {
     int r;         // request, -1: no such tile
@@ -36,13 +60,16 @@ __device__ __forceinline__ int64_t first_tile(const PagedAttnArgs &a, int group,
 
 __device__ __forceinline__ RowTile find_tile(const PagedAttnArgs &a, int group, int unit, int64_t w) {
     RowTile t;
-    int x = 0, y = a.n_seqs - 1;
-    while (x < y) {
-        const int mid = (x + y + 1) >> 1;
-        if (first_tile(a, group, unit, mid) <= w)
-            x = mid;
-        else
-            y = mid - 1;
+    // the last request that begins at or before tile w, 32 candidates a round
+    // (every warp of the block by itself)
+    const int lane = threadIdx.x & 31;
+    int x = 0, n = a.n_seqs;  // among [x, x + n)
+    while (n > 1) {
+        const int step = (n + 31) / 32, i = lane * step;
+        const uint32_t before = __ballot_sync(0xffffffffu, i < n && first_tile(a, group, unit, x + i) <= w);
+        const int k = before ? 31 - __clz(before) : 0;
+        x += k * step;
+        n = min(step, n - k * step);
     }
     t.r = x;
     t.tok0 = min((int64_t)max(a.cu_new[x], 0), a.n_tokens);
@@ -54,6 +81,29 @@ __device__ __forceinline__ RowTile find_tile(const PagedAttnArgs &a, int group, 
     t.row0 = (int)row0;
     t.rows = rows > INT32_MAX ? INT32_MAX : (int)rows;
     return t;
+}
+
+// Maps of k and v as (dim, token, head, page), boxes of 64 dims and
+// min(page_size, keys) tokens, 128-byte swizzle; what lies outside reads as 0.
+cudaError_t paged_cache_maps(const PagedCacheView &c, int keys, CUtensorMap *k, CUtensorMap *v);
+// rows of q as (dim, head, token), boxes of 64 x heads x tokens
+cudaError_t paged_q_map(const PagedAttnArgs &a, int heads, int tokens, CUtensorMap *m);
+// tensor-map strides are below 2^40 bytes and not 0
+bool paged_strides_mappable(const PagedCacheView &c);
+
+// cudaFuncSetAttribute of the dynamic shared memory, once per device
+template <typename F>
+cudaError_t paged_smem_once(F *kernel, int bytes, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+        done[dev].store(true, std::memory_order_release);
+    }
+    return cudaSuccess;
 }
 
 }  // namespace kk

@@ -61,9 +61,13 @@ struct ChunkCfg {
 };
 static_assert(ChunkCfg<128>::SMEM <= 227 * 1024, "shared memory");
 
-// Shared-memory matrix descriptor, 128-byte swizzle (mode 2 in [61,64)).
-__device__ __forceinline__ uint64_t sdesc128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return sdesc(addr, lbo, sbo) | (2ull << 61);
+// Shared-memory matrix descriptors, 128-byte swizzle, as two words: the upper
+// one (SBO 1024 bytes between blocks of 8 rows, version 1 at bit 46, swizzle
+// mode 2 in [61,64)) is the same for all, the lower one is start >> 4 and
+// LBO >> 4 at bit 16, so that a step in shared memory is one 32-bit addition.
+constexpr uint32_t kDescHi = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+    return (addr >> 4 & 0x3FFFu) | (lbo >> 4) << 16;
 }
 
 // Instruction descriptor, kind::f16: D F32, A and B half (0) or bfloat16 (1)
@@ -72,13 +76,37 @@ __device__ __forceinline__ constexpr uint32_t idesc_of(int bf16, int b_rows, int
     return idesc_f16(kTile, n) | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)b_rows << 16;
 }
 
-// D[tmem] (+)= A[tmem] B
-__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// one lane of the warp, the same in every call
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
+// D[tmem] (+)= A[shared] B[shared]
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
+        : "memory");
+}
+
+// D[tmem] (+)= A[tmem] B[shared]
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
         : "memory");
 }
 
@@ -109,14 +137,6 @@ __device__ __forceinline__ void tmem_put32(uint32_t taddr, const uint32_t *r) {
 }
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 2^x, results below 2^-126 as 0 (a weight is at most 2^kGrow and rounded to
-// 16 bits afterwards)
-__device__ __forceinline__ float pow2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
@@ -124,15 +144,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z,
-                                            int w) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-        : "memory");
-}
-
 }  // namespace
 
 template <typename T, int DP>
@@ -181,12 +192,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *sQ = smem, *sKV = smem + 2 * C::TILE_BYTES;
     const uint32_t bars = smem_u32(sKV + kStages * C::TILE_BYTES);
     const uint32_t bQ = bars, bFull = bars + 16, bEmpty = bFull + 8 * kStages, bS = bEmpty + 8 * kStages,
-                   bP = bS + 16, bPV = bP + 16, bDrain = bPV + 16;
+                   bP = bS + 16, bPV = bP + 32, bDrain = bPV + 16;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bQ + 8 * i, 1);
             mbar_init(bS + 8 * i, 1);
-            mbar_init(bP + 8 * i, kTile);
+            mbar_init(bP + 16 * i, 4);      // the four warps of a tile, keys 0-63
+            mbar_init(bP + 16 * i + 8, 4);  // keys 64-127
             mbar_init(bPV + 8 * i, 1);
         }
         for (int i = 0; i < kStages; ++i) {
@@ -239,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int v = 0; v < 2; ++v, ++i) {
                     const uint32_t s = i % kStages;
                     if (lane == 0) {
-                        if (i >= kStages) ok = mbar_wait(bEmpty + 8 * s, (i / kStages - 1) & 1, a.err, kErrPagedWait);
+                        if (i >= kStages) ok = mbar_wait_tight(bEmpty + 8 * s, (i / kStages - 1) & 1, a.err, kErrPagedWait);
                         if (ok) mbar_expect_tx(bFull + 8 * s, C::TILE_BYTES);
                     }
                     ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -259,88 +271,92 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         } else if (warp == kMmaWarp) {
-            const uint32_t id_s = idesc_of(BF16, 0, kTile), id_o = idesc_of(BF16, 1, DP);
+            // The whole warp walks the steps, so that every operand of an MMA
+            // is the same in all lanes and sits in a uniform register; one
+            // elected lane issues. (Issued from code of one lane, an MMA of 64
+            // clocks cost 75-105 clocks of issue.)
+            constexpr uint32_t id_s = idesc_of(BF16, 0, kTile), id_o = idesc_of(BF16, 1, DP);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+            const uint32_t dq = desc_lo(base, 16), dk = desc_lo(base + 2 * C::TILE_BYTES, 16),
+                           dv = desc_lo(base + 2 * C::TILE_BYTES, C::HALF_BYTES);
             bool ok = true;
-            auto full = [&](uint32_t i) {  // tile i of the copy sequence has landed
-                if (ok) ok = mbar_wait(bFull + 8 * (i % kStages), (i / kStages) & 1, a.err, kErrPagedWait);
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                if (ok) ok = mbar_wait_tight(bar, parity, a.err, kErrPagedWait);
                 ok = __all_sync(0xffffffffu, ok);
+                return ok;
             };
-            auto score = [&](int x, int j) {  // S[x] = Q[x] K_j^T
-                if (lane == 0) {
-                    fence_after_sync();
-                    const uint32_t q = smem_u32(sQ + x * C::TILE_BYTES),
-                                   k = smem_u32(sKV + (2 * j) % kStages * C::TILE_BYTES);
+            auto score = [&](int x, uint32_t k) {  // S[x] = Q[x] K^T
+                fence_after_sync();
+                if (elect_one()) {
 #pragma unroll
                     for (int d = 0; d < DP / 16; ++d) {
-                        const uint32_t at = d / 4 * C::HALF_BYTES + d % 4 * 32;
-                        mma_f16(tmem + C::S0 + x * kTile, sdesc128(q + at, 16, 1024), sdesc128(k + at, 16, 1024), id_s,
-                                d > 0);
+                        const uint32_t at = (d / 4 * C::HALF_BYTES + d % 4 * 32) >> 4;
+                        mma_ss(tm + C::S0 + x * kTile, dq + (x * C::TILE_BYTES >> 4) + at, k + at, id_s, d > 0);
                     }
                     mma_commit(bS + 8 * x);
                 }
                 __syncwarp();
             };
-            for (int x = 0; x < 2; ++x)
-                if (n_step[x] > 0) {
-                    if (ok) ok = mbar_wait(bQ + 8 * x, 0, a.err, kErrPagedWait);
-                    full(0);
-                    if (ok) score(x, 0);
-                }
-            if (steps > 0 && ok && lane == 0) mma_commit(bEmpty);
-            for (int j = 0; j < steps && ok; ++j) {
-                const uint32_t iv = 2 * j + 1, ik = 2 * j + 2;  // V_j and K_{j + 1} in the copy sequence
-                full(iv);
-                if (!ok) break;
+            // V_j and K_{j + 1} of the copy sequence: stage and phase
+            uint32_t sv = 1, pv = 0, sk = 2, pk = 0;
+            if (steps > 0) {
+                wait(bFull, 0);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    if (n_step[x] > 0 && wait(bQ + 8 * x, 0)) score(x, dk);
+                if (ok && elect_one()) mma_commit(bEmpty);
+            }
+            const int r_lo = (int)max(min(lo - k0, (int64_t)kTile), (int64_t)0);  // rows of step 0 below the keys
+            for (int j = 0; j < steps && wait(bFull + 8 * sv, pv); ++j) {
                 // the rows of V outside the block's keys become 0
-                const int64_t key0 = k0 + (int64_t)j * kTile;
-                const int r_lo = (int)max(min(lo - key0, (int64_t)kTile), (int64_t)0);
-                const int r_hi = (int)min(k1 - key0, (int64_t)kTile);
-                uint8_t *sv = sKV + iv % kStages * C::TILE_BYTES;
-                if (r_lo > 0 || r_hi < kTile) {
+                const int r_hi = (int)min(k1 - k0 - (int64_t)j * kTile, (int64_t)kTile);
+                if ((j == 0 && r_lo > 0) || r_hi < kTile) {
+                    uint8_t *v = sKV + sv * C::TILE_BYTES;
                     for (int e = lane; e < kTile * HALVES * 8; e += 32) {
                         const int row = (e >> 3) % kTile, h = e / (kTile * 8);
-                        if (row < r_lo || row >= r_hi)
-                            *reinterpret_cast<uint4 *>(sv + h * C::HALF_BYTES + row * 128 + (e & 7) * 16) =
+                        if ((j == 0 && row < r_lo) || row >= r_hi)
+                            *reinterpret_cast<uint4 *>(v + h * C::HALF_BYTES + row * 128 + (e & 7) * 16) =
                                 make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async();
                     __syncwarp();
                 }
-                for (int x = 0; x < 2 && ok; ++x) {
-                    if (j >= n_step[x]) continue;
-                    ok = mbar_wait(bP + 8 * x, j & 1, a.err, kErrPagedWait);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        fence_after_sync();
-                        const uint32_t v = smem_u32(sv);
+                const uint32_t v = dv + sv * (C::TILE_BYTES >> 4);
 #pragma unroll
-                        for (int k = 0; k < kTile / 16; ++k)
-                            mma_f16_ts(tmem + C::O0 + x * DP, tmem + C::P0 + x * C::P_STEP + k * 8,
-                                       sdesc128(v + k * 2048, C::HALF_BYTES, 1024), id_o, j > 0 || k > 0);
-                        mma_commit(bPV + 8 * x);
-                    }
-                    __syncwarp();
-                    if (j + 1 < n_step[x]) {
-                        full(ik);
-                        if (C::P_OVER_S && ok) {
-                            ok = mbar_wait(bPV + 8 * x, j & 1, a.err, kErrPagedWait);
-                            ok = __all_sync(0xffffffffu, ok);
+                for (int x = 0; x < 2; ++x) {
+                    if (j >= n_step[x]) continue;
+                    // O[x] += P V, the first 64 keys as soon as their weights are there
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (!wait(bP + 16 * x + 8 * h, j & 1)) break;
+                        fence_after_sync();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 4 * h; k < 4 * h + 4; ++k)
+                                mma_ts(tm + C::O0 + x * DP, tm + C::P0 + x * C::P_STEP + k * 8, v + (k * 2048 >> 4),
+                                       id_o, j > 0 || k > 0);
+                            if (h == 1) mma_commit(bPV + 8 * x);
                         }
-                        if (ok) score(x, j + 1);
+                        __syncwarp();
                     }
+                    if (!ok) break;
+                    if (j + 1 < n_step[x] && wait(bFull + 8 * sk, pk) && (!C::P_OVER_S || wait(bPV + 8 * x, j & 1)))
+                        score(x, dk + sk * (C::TILE_BYTES >> 4));
                 }
-                if (ok && lane == 0) {
-                    mma_commit(bEmpty + 8 * (iv % kStages));
-                    if (j + 1 < steps) mma_commit(bEmpty + 8 * (ik % kStages));
+                if (!ok) break;
+                if (elect_one()) {
+                    mma_commit(bEmpty + 8 * sv);
+                    if (j + 1 < steps) mma_commit(bEmpty + 8 * sk);
                 }
+                __syncwarp();
+                sv = sv + 2 >= kStages ? (pv ^= 1, sv + 2 - kStages) : sv + 2;
+                sk = sk + 2 >= kStages ? (pk ^= 1, sk + 2 - kStages) : sk + 2;
             }
             // every MMA issued has completed before tensor memory is freed
-            if (lane == 0) {
-                mma_commit(bDrain);
-                mbar_wait(bDrain, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
-            }
+            if (elect_one()) mma_commit(bDrain);
             __syncwarp();
+            mbar_wait(bDrain, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
         }
         asm volatile("bar.sync 0;" ::: "memory");
         if (warp == kMmaWarp) {
@@ -357,10 +373,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = i < n_tok[x] && row < tile_tok * group;
         const int64_t tq = t.tok0 + tok[x] + i;
         const int head = kvh * group + row % group;
-        // the keys this row sees, [see_lo, see_hi)
+        // the keys this row sees, [see_lo, see_hi), counted from k0
         const int64_t pos = (int64_t)t.base + tok[x] + i;
-        const int64_t see_hi = live ? min(min(pos + 1, cap), k1) : 0;
-        const int64_t see_lo = a.window > 0 ? pos - a.window + 1 : 0;
+        const int see_hi = live ? (int)(min(min(pos + 1, cap), k1) - k0) : 0;
+        const int see_lo = a.window > 0 ? (int)(pos - a.window + 1 - k0) : 0;
         // scores in base 2; a negative scale is the positive one of -S, and a
         // scale of 0 a tiny one (masked scores are -inf, and 0 inf is a NaN)
         const float sc = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
@@ -368,23 +384,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         const int n = n_step[x];
+        // pages of a step that are missing, a bit each: the lane's page of the
+        // next step is read a step ahead
+        const int shift = 31 - __clz(min(page_size, kTile));
+        auto page_gone = [&](int j) {
+            const int64_t key = k0 + (int64_t)j * kTile + ((int64_t)lane << shift);
+            if (lane >= kTile >> shift || key >= k1 || j >= n) return false;
+            const int page = table[(int)key / page_size];
+            return page < 0 || page >= a.cache.n_pages;
+        };
+        bool gone = page_gone(0);
         for (int j = 0; j < n && ok; ++j) {
-            const int64_t key0 = k0 + (int64_t)j * kTile;
-            // pages of this step that are missing, a bit each
-            const int shift = 31 - __clz(min(page_size, kTile)), boxes = kTile >> shift;
-            bool gone = false;
-            {
-                const int64_t key = key0 + ((int64_t)lane << shift);
-                if (lane < boxes && key < k1) {
-                    const int page = table[(int)key / page_size];
-                    gone = page < 0 || page >= a.cache.n_pages;
-                }
-            }
+            const int c0 = see_lo - j * kTile, c1 = see_hi - j * kTile;  // the columns seen, [c0, c1)
             const uint32_t missing = __ballot_sync(0xffffffffu, gone);
-            ok = mbar_wait(bS + 8 * x, j & 1, a.err, kErrPagedWait);
+            gone = page_gone(j + 1);
+            ok = mbar_wait_tight(bS + 8 * x, j & 1, a.err, kErrPagedWait);
             // the product of the step before is complete too (P_OVER_S: the
             // issuer waited for it); its barrier's phases are taken in turn
-            if (!C::P_OVER_S && j > 0 && ok) ok = mbar_wait(bPV + 8 * x, (j - 1) & 1, a.err, kErrPagedWait);
+            if (!C::P_OVER_S && j > 0 && ok) ok = mbar_wait_tight(bPV + 8 * x, (j - 1) & 1, a.err, kErrPagedWait);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after_sync();
@@ -397,16 +414,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < kTile; ++c) s[c] = -s[c];
             }
             // masked scores
-            if (key0 < see_lo || key0 + kTile > see_hi || missing) {
-                const int c0 = (int)max(min(see_lo - key0, (int64_t)kTile), (int64_t)0),
-                          c1 = (int)max(min(see_hi - key0, (int64_t)kTile), (int64_t)0);
+            if (c0 > 0 || c1 < kTile || missing) {
 #pragma unroll
                 for (int c = 0; c < kTile; ++c)
                     if (c < c0 || c >= c1) s[c] = -INFINITY;
                 if (missing) {
 #pragma unroll
-                    for (int c = 0; c < kTile; ++c)
-                        if (missing >> (c >> shift) & 1) s[c] = -INFINITY;
+                    for (int w = 0; w < kTile; w += 32) {
+                        uint32_t hide = 0;  // a bit per column, from the bits of its blocks of 8
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8)
+                            if (missing >> ((w + c) >> shift) & 1) hide |= 0xffu << c;
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (hide >> c & 1) s[w + c] = -INFINITY;
+                    }
                 }
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
@@ -446,16 +468,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     u[e] = pack2(p.x, p.y, T());
                 }
                 tmem_put32(tP + c / 2, u);
+                tmem_put_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bP + 16 * x + c / 8);
             }
             l += add.x + add.y;
-            tmem_put_wait();
-            fence_before_sync();
-            mbar_arrive(bP + 8 * x);
         }
-        if (n > 0 && ok) ok = mbar_wait(bPV + 8 * x, (n - 1) & 1, a.err, kErrPagedWait);
+        if (n > 0 && ok) ok = mbar_wait_tight(bPV + 8 * x, (n - 1) & 1, a.err, kErrPagedWait);
         ok = __all_sync(0xffffffffu, ok);
         fence_after_sync();
-        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a NaN sum stays one
+        const float inv = paged_inverse(l);
         const int64_t part = (tq * a.n_heads + head) * a.splits + sp;
         if (n_pieces > 1 && live && ok) a.part_ml[part] = make_float2(n > 0 ? m * sc : -INFINITY, l);
 #pragma unroll
@@ -518,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     acc.x += f * o.x, acc.y += f * o.y, acc.z += f * o.z, acc.w += f * o.w;
                 }
             }
-            const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+            const float inv = paged_inverse(l);
             if (lane * 4 < D)
                 *reinterpret_cast<uint2 *>((T *)a.out + tq * a.out_stride + (int64_t)head * D + lane * 4) =
                     make_uint2(pack2(acc.x * inv, acc.y * inv, T()), pack2(acc.z * inv, acc.w * inv, T()));
@@ -545,72 +568,79 @@ static cudaError_t encoder(PFN_cuTensorMapEncodeTiled_v12000 *out) {
     return cudaSuccess;
 }
 
-// Swizzled tiles are made of blocks of 8 rows: a step's 128 keys are whole
-// pages of 8, 16, 32, 64 or 128 tokens, or lie in one page of a multiple of
-// 128. Tensor-map strides are below 2^40 bytes and not 0.
-bool paged_chunk_serves(const PagedCacheView &c, int n_heads) {
-    const bool page = c.page_size >= 8 && (kTile % c.page_size == 0 || c.page_size % kTile == 0);
+bool paged_strides_mappable(const PagedCacheView &c) {
     const int64_t most = (int64_t)1 << 39;
-    return page && n_heads / c.n_kv_heads <= kTile && c.token_stride > 0 && c.token_stride < most &&
-           c.head_stride > 0 && c.head_stride < most && c.page_stride > 0 && c.page_stride < most;
+    return c.token_stride > 0 && c.token_stride < most && c.head_stride > 0 && c.head_stride < most &&
+           c.page_stride > 0 && c.page_stride < most;
 }
 
-int paged_chunk_unit(int group) { return 2 * (kTile / group) * group; }
+static CUtensorMapDataType map_type(int bf16) {
+    return bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
 
-static bool cache_map(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap *m, const PagedCacheView &c,
-                      const void *base) {
+cudaError_t paged_cache_maps(const PagedCacheView &c, int keys, CUtensorMap *k, CUtensorMap *v) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode;
+    const cudaError_t e = encoder(&encode);
+    if (e != cudaSuccess) return e;
     const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv_heads,
                                 (cuuint64_t)c.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)c.token_stride * 2, (cuuint64_t)c.head_stride * 2,
                                    (cuuint64_t)c.page_stride * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(c.page_size < kTile ? c.page_size : kTile), 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(c.page_size < keys ? c.page_size : keys), 1, 1};
     const cuuint32_t step[4] = {1, 1, 1, 1};
-    return encode(m, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void *)base, dims,
-                  strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    for (int i = 0; i < 2; ++i)
+        if (encode(i ? v : k, map_type(c.bf16), 4, i ? c.v : c.k, dims, strides, box, step,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    return cudaSuccess;
 }
 
-template <typename T, int DP>
-static cudaError_t launch_chunk(const PagedAttnArgs &a, int64_t tiles, const CUtensorMap &q, const CUtensorMap &k,
-                                const CUtensorMap &v, cudaStream_t st) {
-    static std::atomic<bool> attr[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+cudaError_t paged_q_map(const PagedAttnArgs &a, int heads, int tokens, CUtensorMap *m) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode;
+    const cudaError_t e = encoder(&encode);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!attr[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(k_paged_attn_chunk<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 ChunkCfg<DP>::SMEM);
-        if (e != cudaSuccess) return e;
-        attr[dev].store(true, std::memory_order_release);
-    }
+    const cuuint64_t dims[3] = {(cuuint64_t)a.cache.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.cache.head_dim * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)tokens};
+    const cuuint32_t step[3] = {1, 1, 1};
+    return encode(m, map_type(a.cache.bf16), 3, (void *)a.q, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+// Swizzled tiles are made of blocks of 8 rows: a step's 128 keys are whole
+// pages of 8, 16, 32, 64 or 128 tokens, or lie in one page of a multiple of
+// 128.
+bool paged_chunk_serves(const PagedCacheView &c, int n_heads) {
+    const bool page = c.page_size >= 8 && (kTile % c.page_size == 0 || c.page_size % kTile == 0);
+    return page && n_heads / c.n_kv_heads <= kTile && paged_strides_mappable(c);
+}
+
+int paged_chunk_unit(int group) { return 2 * (kTile / group) * group; }
+
+template <typename T, int DP>
+static cudaError_t launch_chunk(const PagedAttnArgs &a, cudaStream_t st) {
+    static std::atomic<bool> attr[64];
+    cudaError_t e = paged_smem_once(k_paged_attn_chunk<T, DP>, ChunkCfg<DP>::SMEM, attr);
+    if (e != cudaSuccess) return e;
+    const int group = a.n_heads / a.cache.n_kv_heads, tile_tok = kTile / group;
+    CUtensorMap q, k, v;
+    e = paged_q_map(a, group, tile_tok, &q);
+    if (e == cudaSuccess) e = paged_cache_maps(a.cache, kTile, &k, &v);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = a.n_tokens / (2 * tile_tok) + a.n_seqs;
     const dim3 grid((unsigned)tiles, (unsigned)a.cache.n_kv_heads, (unsigned)a.splits);
     k_paged_attn_chunk<T, DP><<<grid, kThreads, ChunkCfg<DP>::SMEM, st>>>(a, q, k, v);
     return cudaGetLastError();
 }
 
 cudaError_t paged_chunk_attn(const PagedAttnArgs &a, cudaStream_t st) {
-    const PagedCacheView &c = a.cache;
-    const int group = a.n_heads / c.n_kv_heads, tile_tok = kTile / group;
-    PFN_cuTensorMapEncodeTiled_v12000 encode;
-    cudaError_t e = encoder(&encode);
-    if (e != cudaSuccess) return e;
-    CUtensorMap mq, mk, mv;
-    const cuuint64_t dims[3] = {(cuuint64_t)c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
-    const cuuint64_t strides[2] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)a.q_stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)tile_tok};
-    const cuuint32_t step[3] = {1, 1, 1};
-    if (encode(&mq, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void *)a.q, dims,
-               strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
-        !cache_map(encode, &mk, c, c.k) || !cache_map(encode, &mv, c, c.v))
-        return cudaErrorInvalidValue;
-    const int64_t tiles = a.n_tokens / (2 * tile_tok) + a.n_seqs;
-    if (c.head_dim <= 64)
-        return c.bf16 ? launch_chunk<__nv_bfloat16, 64>(a, tiles, mq, mk, mv, st)
-                      : launch_chunk<__half, 64>(a, tiles, mq, mk, mv, st);
-    return c.bf16 ? launch_chunk<__nv_bfloat16, 128>(a, tiles, mq, mk, mv, st)
-                  : launch_chunk<__half, 128>(a, tiles, mq, mk, mv, st);
+    if (a.cache.head_dim <= 64)
+        return a.cache.bf16 ? launch_chunk<__nv_bfloat16, 64>(a, st) : launch_chunk<__half, 64>(a, st);
+    return a.cache.bf16 ? launch_chunk<__nv_bfloat16, 128>(a, st) : launch_chunk<__half, 128>(a, st);
 }
 
 }  // namespace kk

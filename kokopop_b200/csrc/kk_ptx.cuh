@@ -60,6 +60,24 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int *er
     }
 }
 
+// The same for waits between the roles of a step, where the reaction counts:
+// the clock is read once in 256 tries, not between any two.
+__device__ __forceinline__ bool mbar_wait_tight(uint32_t bar, uint32_t parity, int *err, int code,
+                                                unsigned long long limit_ns = TC_WAIT_NS) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try(bar, parity)) return true;
+        if ((i & 255) == 0) {
+            const uint64_t now = globaltimer();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > limit_ns) {
+                atomicCAS(err, 0, code);
+                return false;
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),

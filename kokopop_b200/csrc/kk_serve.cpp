@@ -172,13 +172,13 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         a.err = (int *)ctx->d_err.p;
         // pieces of the key axis: enough blocks for about four rounds of the
         // row kernel's two blocks on each of 148 SMs (the chunk kernel: two
-        // rounds of its one), 128 keys or more each
+        // rounds of its one), 256 keys or more each
         const int64_t rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
         const int64_t blocks = std::min(plan.tiles, n_seqs * ((rows + plan.unit - 1) / plan.unit)) * a.cache.n_kv_heads;
         int64_t keys = std::max(max_len, 1);
         if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + plan.unit / group + 16);
         const int64_t want = plan.chunk ? 296 : 1184, step = plan.chunk ? 128 : 64;
-        const int64_t splits = std::min((want + blocks - 1) / blocks, (keys + 127) / 128);
+        const int64_t splits = std::min((want + blocks - 1) / blocks, (keys + 255) / 256);
         a.splits = capturing(st) ? 1 : (int)std::min<int64_t>(splits, 256);
         a.split_keys = (int)(((keys + a.splits - 1) / a.splits + step - 1) / step * step);
         if (a.splits == 1) {
