@@ -406,7 +406,8 @@ struct PagedAttnArgs {
     int splits, split_keys;
     float *part_o;   // [n_tokens][n_heads][splits][head_dim]
     float2 *part_ml; // [n_tokens][n_heads][splits] running maximum (base 2) and sum
-    unsigned *count; // [tiles][n_kv_heads], zero between launches
+    unsigned *count; // row kernel: [tiles][n_kv_heads], zero between launches
+    int *part_n;     // chunk kernel: [n_tokens][n_heads], pieces of a row
     int *err;        // device error word
 };
 // How a call is divided: the tensor-memory kernel (chunks of queries) or the

@@ -15,10 +15,10 @@
 // has grown by more than 8 in base 2 (the weights stay below 2^8), which after
 // the first steps is rare; the result does not depend on m but for rounding.
 //
-// Roles: warps 0-3 and 4-7 softmax and output of the two tiles, warp 8 issues
-// the tcgen05.mma, warp 9 the copies (10 and 11 only fill their warpgroup). Keys and values come page by page
-// through 4-D tensor maps (dim, token, head, page) into 128-byte swizzled
-// tiles, so any stride order of the cache is served; pages that are missing or
+// Roles: warps 0-3 and 4-7 softmax and output of the two tiles, warps 8 and 10
+// issue their tcgen05.mma, warp 9 the copies (11 only fills its warpgroup).
+// Keys and values come page by page through 4-D tensor maps (dim, token, head,
+// page) into 128-byte swizzled tiles, so any stride order of the cache is served; pages that are missing or
 // hold no key of the tile are fetched from outside the tensor and read as
 // zeros. Values of tokens outside the block's key range may be anything, and 0
 // times a NaN is one: their rows are zeroed in shared memory in the steps at
@@ -41,19 +41,19 @@ namespace kk {
 namespace {
 
 constexpr int kTile = 128;       // rows of a tile, keys of a step
-constexpr int kStages = 5;       // K or V tiles in flight
+constexpr int kStages = 2;       // pairs of a V tile and the next step's K tile
 constexpr int kThreads = 384;
 // registers of a thread: 168 at launch (3 warpgroups), moved from the copy and
-// MMA warpgroup to the two that hold a row of scores: 56 + 2 x 224 = 3 x 168
-constexpr int kRegsFew = 56, kRegsMany = 224;
-constexpr int kMmaWarp = 8, kCopyWarp = 9;
+// MMA warpgroup to the two that hold a row of scores: 88 + 2 x 208 = 3 x 168
+constexpr int kRegsFew = 88, kRegsMany = 208;
+constexpr int kMmaWarp = 8, kCopyWarp = 9, kMmaWarp1 = 10;
 constexpr float kGrow = 8.0f;    // base-2 growth of a maximum that is left alone
 
 template <int DP>
 struct ChunkCfg {
     static constexpr int TILE_BYTES = kTile * DP * 2;
     static constexpr int HALF_BYTES = kTile * 128;   // 64 dims of a tile
-    static constexpr int SMEM = (2 + kStages) * TILE_BYTES + 1024 /*barriers*/ + 1024 /*align*/;
+    static constexpr int SMEM = (2 + 2 * kStages) * TILE_BYTES + 1024 /*barriers*/ + 1024 /*align*/;
     static constexpr bool P_OVER_S = DP > 64;
     // tensor memory columns
     static constexpr int S0 = 0, O0 = 2 * kTile, P0 = P_OVER_S ? 0 : O0 + 2 * DP, P_STEP = P_OVER_S ? kTile : kTile / 2;
@@ -85,6 +85,20 @@ __device__ __forceinline__ bool elect_one() {
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(p));
     return p != 0;
+}
+
+// Whether v holds in any of the 256 softmax threads (named barrier 1).
+__device__ __forceinline__ bool any_of_barrier(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
 }
 
 // D[tmem] (+)= A[shared] B[shared]
@@ -156,7 +170,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint32_t tmem_s;
-    __shared__ unsigned last_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = a.n_heads / a.cache.n_kv_heads, kvh = blockIdx.y, D = a.cache.head_dim;
     const int tile_tok = kTile / group;  // tokens of a tile
@@ -190,9 +203,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int page_size = a.cache.page_size;
 
     uint8_t *sQ = smem, *sKV = smem + 2 * C::TILE_BYTES;
-    const uint32_t bars = smem_u32(sKV + kStages * C::TILE_BYTES);
+    const uint32_t bars = smem_u32(sKV + 2 * kStages * C::TILE_BYTES);
     const uint32_t bQ = bars, bFull = bars + 16, bEmpty = bFull + 8 * kStages, bS = bEmpty + 8 * kStages,
-                   bP = bS + 16, bPV = bP + 32, bDrain = bPV + 16;
+                   bP = bS + 16, bPV = bP + 32, bDrain = bPV + 16, bZero = bDrain + 16, bTurn = bZero + 8;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bQ + 8 * i, 1);
@@ -203,9 +216,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < kStages; ++i) {
             mbar_init(bFull + 8 * i, 1);
-            mbar_init(bEmpty + 8 * i, 1);
+            mbar_init(bEmpty + 8 * i, 2);  // the issuers of both tiles
         }
         mbar_init(bDrain, 1);
+        mbar_init(bDrain + 8, 1);
+        mbar_init(bZero, 2);
+        mbar_init(bTurn, 4);      // the softmax warps of a tile
+        mbar_init(bTurn + 8, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -224,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
         if (warp == kCopyWarp) {
-            // Q of both tiles, then K and V of each step: tile i of the sequence
-            // K 0, V 0, K 1, V 1, ... goes to stage i % kStages
+            // Q of both tiles, then pair i = (V of step i - 1, K of step i) into
+            // stage i % kStages; the first has no V, the last no K
             if (lane == 0)
                 for (int x = 0; x < 2; ++x)
                     if (n_step[x] > 0) {
@@ -237,83 +254,95 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int box = min(page_size, kTile);           // tokens of a copy
             const int boxes = kTile / box;                   // copies of 64 dims of a tile
             const int part = lane % boxes, half = lane / boxes;
+            const int pairs = steps > 0 ? steps + 1 : 0;
+            int page = -1, off = 0;  // of the K of the pair before, the V of this one
             bool ok = true;
-            uint32_t i = 0;
-            for (int j = 0; j < steps && ok; ++j) {
-                const int64_t key = k0 + (int64_t)j * kTile + part * box;
-                int page = -1, off = 0;
+            int i = 0;
+            for (; i < pairs; ++i) {
+                const int page_v = page, off_v = off;
+                const int64_t key = k0 + (int64_t)i * kTile + part * box;
+                page = -1;
                 if (half < HALVES && key < k1 && key + box > lo) {
                     const int col = (int)key / page_size;
                     page = table[col];
                     off = (int)key - col * page_size;
                     if (page < 0 || page >= a.cache.n_pages) page = -1;
                 }
-                for (int v = 0; v < 2; ++v, ++i) {
-                    const uint32_t s = i % kStages;
-                    if (lane == 0) {
-                        if (i >= kStages) ok = mbar_wait_tight(bEmpty + 8 * s, (i / kStages - 1) & 1, a.err, kErrPagedWait);
-                        if (ok) mbar_expect_tx(bFull + 8 * s, C::TILE_BYTES);
-                    }
-                    ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                    if (!ok) break;
-                    if (half < HALVES)
-                        tma_load_4d(smem_u32(sKV + s * C::TILE_BYTES + half * C::HALF_BYTES + part * box * 128),
-                                    v ? &map_v : &map_k, bFull + 8 * s, 64 * half, off, kvh, page);
+                const int s = i % kStages;
+                const uint32_t bar = bFull + 8 * s, at = smem_u32(sKV + 2 * s * C::TILE_BYTES);
+                if (lane == 0) {
+                    if (i >= kStages) ok = mbar_wait_tight(bEmpty + 8 * s, (i / kStages - 1) & 1, a.err, kErrPagedWait);
+                    if (ok) mbar_expect_tx(bar, (i > 0 && i < steps ? 2 : 1) * C::TILE_BYTES);
+                }
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                if (!ok) break;
+                if (half < HALVES) {
+                    const uint32_t to = at + half * C::HALF_BYTES + part * box * 128;
+                    if (i > 0) tma_load_4d(to, &map_v, bar, 64 * half, off_v, kvh, page_v);
+                    if (i < steps) tma_load_4d(to + C::TILE_BYTES, &map_k, bar, 64 * half, off, kvh, page);
                 }
             }
             // the last copy into each stage has landed (consumed already, unless
             // a wait ran out)
             if (lane == 0) {
-                for (uint32_t c = i > kStages ? i - kStages : 0; c < i; ++c)
+                for (int c = max(i - kStages, 0); c < i; ++c)
                     mbar_wait(bFull + 8 * (c % kStages), (c / kStages) & 1, a.err, kErrPagedWait, TC_DRAIN_NS);
                 for (int x = 0; x < 2; ++x)
                     if (n_step[x] > 0) mbar_wait(bQ + 8 * x, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
             }
             __syncwarp();
-        } else if (warp == kMmaWarp) {
+        } else if (warp == kMmaWarp || warp == kMmaWarp1) {
+            // A warp per tile, so that neither waits for the other's softmax.
             // The whole warp walks the steps, so that every operand of an MMA
             // is the same in all lanes and sits in a uniform register; one
             // elected lane issues. (Issued from code of one lane, an MMA of 64
             // clocks cost 75-105 clocks of issue.)
             constexpr uint32_t id_s = idesc_of(BF16, 0, kTile), id_o = idesc_of(BF16, 1, DP);
+            const int x = __shfl_sync(0xffffffffu, warp == kMmaWarp ? 0 : 1, 0);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
-            const uint32_t dq = desc_lo(base, 16), dk = desc_lo(base + 2 * C::TILE_BYTES, 16),
-                           dv = desc_lo(base + 2 * C::TILE_BYTES, C::HALF_BYTES);
+            const uint32_t q = desc_lo(base + x * C::TILE_BYTES, 16);
+            const uint32_t dv = desc_lo(base + 2 * C::TILE_BYTES, C::HALF_BYTES),
+                           dk = desc_lo(base + 3 * C::TILE_BYTES, 16);
+            const uint32_t tS = tm + C::S0 + x * kTile, tO = tm + C::O0 + x * DP, tP = tm + C::P0 + x * C::P_STEP;
+            const int n = __shfl_sync(0xffffffffu, x ? n_step[1] : n_step[0], 0);
+            const int all = __shfl_sync(0xffffffffu, steps, 0);
             bool ok = true;
+            uint32_t zeroed = 0;
             auto wait = [&](uint32_t bar, uint32_t parity) {
-                if (ok) ok = mbar_wait_tight(bar, parity, a.err, kErrPagedWait);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = __all_sync(0xffffffffu, mbar_wait_tight(bar, parity, a.err, kErrPagedWait));
                 return ok;
             };
-            auto score = [&](int x, uint32_t k) {  // S[x] = Q[x] K^T
+            auto score = [&](uint32_t k, int s) {  // S = Q K^T, K in stage s
                 fence_after_sync();
                 if (elect_one()) {
 #pragma unroll
                     for (int d = 0; d < DP / 16; ++d) {
                         const uint32_t at = (d / 4 * C::HALF_BYTES + d % 4 * 32) >> 4;
-                        mma_ss(tm + C::S0 + x * kTile, dq + (x * C::TILE_BYTES >> 4) + at, k + at, id_s, d > 0);
+                        mma_ss(tS, q + at, k + at, id_s, d > 0);
                     }
                     mma_commit(bS + 8 * x);
+                    mma_commit(bEmpty + 8 * s);
                 }
                 __syncwarp();
             };
-            // V_j and K_{j + 1} of the copy sequence: stage and phase
-            uint32_t sv = 1, pv = 0, sk = 2, pk = 0;
-            if (steps > 0) {
-                wait(bFull, 0);
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    if (n_step[x] > 0 && wait(bQ + 8 * x, 0)) score(x, dk);
-                if (ok && elect_one()) mma_commit(bEmpty);
-            }
             const int r_lo = (int)max(min(lo - k0, (int64_t)kTile), (int64_t)0);  // rows of step 0 below the keys
-            for (int j = 0; j < steps && wait(bFull + 8 * sv, pv); ++j) {
+            if (all > 0 && wait(bFull, 0)) {
+                if (n > 0) {
+                    if (wait(bQ + 8 * x, 0)) score(dk, 0);
+                } else if (elect_one()) {
+                    mbar_arrive(bEmpty);
+                }
+            }
+            __syncwarp();
+            for (int j = 0; j < all && ok; ++j) {
+                const int s = (j + 1) % kStages;
+                if (!wait(bFull + 8 * s, (j + 1) / kStages & 1)) break;
                 // the rows of V outside the block's keys become 0
                 const int r_hi = (int)min(k1 - k0 - (int64_t)j * kTile, (int64_t)kTile);
                 if ((j == 0 && r_lo > 0) || r_hi < kTile) {
-                    uint8_t *v = sKV + sv * C::TILE_BYTES;
-                    for (int e = lane; e < kTile * HALVES * 8; e += 32) {
+                    uint8_t *v = sKV + 2 * s * C::TILE_BYTES;
+                    for (int e = lane + 32 * x; e < kTile * HALVES * 8; e += 64) {
                         const int row = (e >> 3) % kTile, h = e / (kTile * 8);
                         if ((j == 0 && row < r_lo) || row >= r_hi)
                             *reinterpret_cast<uint4 *>(v + h * C::HALF_BYTES + row * 128 + (e & 7) * 16) =
@@ -321,42 +350,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     fence_proxy_async();
                     __syncwarp();
+                    if (elect_one()) mbar_arrive(bZero);  // both issuers' halves, bounded like every wait
+                    if (!wait(bZero, zeroed++ & 1)) break;
                 }
-                const uint32_t v = dv + sv * (C::TILE_BYTES >> 4);
+                if (j >= n) {  // this tile has no such step: only the stage is given back
+                    if (elect_one()) mbar_arrive(bEmpty + 8 * s);
+                    __syncwarp();
+                    continue;
+                }
+                const uint32_t at = 2 * s * (C::TILE_BYTES >> 4);
+                // O += P V, the first 64 keys as soon as their weights are there
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (j >= n_step[x]) continue;
-                    // O[x] += P V, the first 64 keys as soon as their weights are there
+                for (int h = 0; h < 2; ++h) {
+                    if (!wait(bP + 16 * x + 8 * h, j & 1)) break;
+                    fence_after_sync();
+                    if (elect_one()) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (!wait(bP + 16 * x + 8 * h, j & 1)) break;
-                        fence_after_sync();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = 4 * h; k < 4 * h + 4; ++k)
-                                mma_ts(tm + C::O0 + x * DP, tm + C::P0 + x * C::P_STEP + k * 8, v + (k * 2048 >> 4),
-                                       id_o, j > 0 || k > 0);
-                            if (h == 1) mma_commit(bPV + 8 * x);
+                        for (int k = 4 * h; k < 4 * h + 4; ++k)
+                            mma_ts(tO, tP + k * 8, dv + at + (k * 2048 >> 4), id_o, j > 0 || k > 0);
+                        if (h == 1) {
+                            mma_commit(bPV + 8 * x);
+                            if (j + 1 >= n) mma_commit(bEmpty + 8 * s);
                         }
-                        __syncwarp();
                     }
-                    if (!ok) break;
-                    if (j + 1 < n_step[x] && wait(bFull + 8 * sk, pk) && (!C::P_OVER_S || wait(bPV + 8 * x, j & 1)))
-                        score(x, dk + sk * (C::TILE_BYTES >> 4));
+                    __syncwarp();
                 }
-                if (!ok) break;
-                if (elect_one()) {
-                    mma_commit(bEmpty + 8 * sv);
-                    if (j + 1 < steps) mma_commit(bEmpty + 8 * sk);
-                }
-                __syncwarp();
-                sv = sv + 2 >= kStages ? (pv ^= 1, sv + 2 - kStages) : sv + 2;
-                sk = sk + 2 >= kStages ? (pk ^= 1, sk + 2 - kStages) : sk + 2;
+                if (ok && j + 1 < n && (!C::P_OVER_S || wait(bPV + 8 * x, j & 1))) score(dk + at, s);
             }
             // every MMA issued has completed before tensor memory is freed
-            if (elect_one()) mma_commit(bDrain);
+            if (elect_one()) mma_commit(bDrain + 8 * x);
             __syncwarp();
-            mbar_wait(bDrain, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
+            mbar_wait(bDrain + 8 * x, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
         }
         asm volatile("bar.sync 0;" ::: "memory");
         if (warp == kMmaWarp) {
@@ -383,21 +407,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool flip = a.scale < 0.f;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        const int n = n_step[x];
-        // pages of a step that are missing, a bit each: the lane's page of the
-        // next step is read a step ahead
-        const int shift = 31 - __clz(min(page_size, kTile));
-        auto page_gone = [&](int j) {
-            const int64_t key = k0 + (int64_t)j * kTile + ((int64_t)lane << shift);
-            if (lane >= kTile >> shift || key >= k1 || j >= n) return false;
+        const int n = x ? n_step[1] : n_step[0], n_other = x ? n_step[0] : n_step[1];
+        // whether a page of the block's keys is missing, looked up while the
+        // first copies are under way
+        bool gone = false;
+        for (int64_t key = k0 / page_size * page_size + (int64_t)tid * page_size; key < k1;
+             key += (int64_t)2 * kTile * page_size) {
             const int page = table[(int)key / page_size];
-            return page < 0 || page >= a.cache.n_pages;
-        };
-        bool gone = page_gone(0);
+            gone |= page < 0 || page >= a.cache.n_pages;
+        }
+        const bool any_missing = any_of_barrier(gone);
         for (int j = 0; j < n && ok; ++j) {
             const int c0 = see_lo - j * kTile, c1 = see_hi - j * kTile;  // the columns seen, [c0, c1)
-            const uint32_t missing = __ballot_sync(0xffffffffu, gone);
-            gone = page_gone(j + 1);
             ok = mbar_wait_tight(bS + 8 * x, j & 1, a.err, kErrPagedWait);
             // the product of the step before is complete too (P_OVER_S: the
             // issuer waited for it); its barrier's phases are taken in turn
@@ -414,23 +435,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < kTile; ++c) s[c] = -s[c];
             }
             // masked scores
-            if (c0 > 0 || c1 < kTile || missing) {
+            if (c0 > 0 || c1 < kTile || any_missing) {
 #pragma unroll
                 for (int c = 0; c < kTile; ++c)
                     if (c < c0 || c >= c1) s[c] = -INFINITY;
-                if (missing) {
+                if (any_missing) {
 #pragma unroll
                     for (int w = 0; w < kTile; w += 32) {
-                        uint32_t hide = 0;  // a bit per column, from the bits of its blocks of 8
-#pragma unroll
-                        for (int c = 0; c < 32; c += 8)
-                            if (missing >> ((w + c) >> shift) & 1) hide |= 0xffu << c;
+                        uint32_t hide = 0;  // pages are whole blocks of 8 keys
+                        const int key = (int)k0 + j * kTile + w;
+                        for (int c = 0; c < 32 && key + c < k1; c += 8) {
+                            const int page = table[(key + c) / page_size];
+                            if (page < 0 || page >= a.cache.n_pages) hide |= 0xffu << c;
+                        }
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
                             if (hide >> c & 1) s[w + c] = -INFINITY;
                     }
                 }
             }
+            // The softmax of the two tiles takes turns, A 0, B 0, A 1, ...: in
+            // step with one another, both tiles would wait for the tensor
+            // cores at the same time, and then both for the exponentials.
+            if (ok && (x ? j < n_other : j > 0 && j - 1 < n_other))
+                ok = mbar_wait_tight(bTurn + 8 * (x ^ 1), (x ? j : j - 1) & 1, a.err, kErrPagedWait);
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
             for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
@@ -468,6 +496,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     u[e] = pack2(p.x, p.y, T());
                 }
                 tmem_put32(tP + c / 2, u);
+                if (c > 0) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bTurn + 8 * x);
+                }
                 tmem_put_wait();
                 fence_before_sync();
                 __syncwarp();
@@ -480,6 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_after_sync();
         const float inv = paged_inverse(l);
         const int64_t part = (tq * a.n_heads + head) * a.splits + sp;
+        if (a.splits > 1 && live && sp == 0) a.part_n[tq * a.n_heads + head] = n_pieces;
         if (n_pieces > 1 && live && ok) a.part_ml[part] = make_float2(n > 0 ? m * sc : -INFINITY, l);
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
@@ -511,42 +544,41 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         fence_before_sync();
-        if (n_pieces > 1) __threadfence();
         asm volatile("bar.sync 0;" ::: "memory");
-        if (n_pieces == 1) return;
+    }
+}
 
-        // join the pieces: the block that arrives last, a warp per row
-        unsigned *count = a.count + (int64_t)blockIdx.x * gridDim.y + kvh;
-        if (tid == 0) last_s = atomicAdd(count, 1u) == (unsigned)n_pieces - 1;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (!last_s) return;
-        __threadfence();
-        if (tid == 0) *count = 0;
-        const int rows = (n_tok[0] + n_tok[1]) * group;
-        for (int row = warp; row < rows; row += kMmaWarp) {
-            const int64_t tq = t.tok0 + tok_first + row / group;
-            const int head = kvh * group + row % group;
-            const int64_t part = (tq * a.n_heads + head) * a.splits;
-            float top = -INFINITY;
-            for (int s = 0; s < n_pieces; ++s) top = fmaxf(top, __ldcg(&a.part_ml[part + s]).x);
-            const float ref = top == -INFINITY ? 0.f : top;
-            float l = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int s = 0; s < n_pieces; ++s) {
-                const float2 ml = __ldcg(&a.part_ml[part + s]);
-                const float f = exp2f(ml.x - ref);
-                l += f * ml.y;
-                if (lane * 4 < D) {
-                    const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part_o + (part + s) * D) + lane);
-                    acc.x += f * o.x, acc.y += f * o.y, acc.z += f * o.z, acc.w += f * o.w;
-                }
-            }
-            const float inv = paged_inverse(l);
-            if (lane * 4 < D)
-                *reinterpret_cast<uint2 *>((T *)a.out + tq * a.out_stride + (int64_t)head * D + lane * 4) =
-                    make_uint2(pack2(acc.x * inv, acc.y * inv, T()), pack2(acc.z * inv, acc.w * inv, T()));
+// Joins the pieces of the chunk kernel, a warp per (token, head), in the order
+// of the pieces. Rows that one block finished have n = 1 and are left.
+template <typename T>
+__global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
+    const int lane = threadIdx.x & 31, D = a.cache.head_dim;
+    const int64_t row = blockIdx.x * 8ll + (threadIdx.x >> 5), tok = row / a.n_heads;
+    if (tok >= min((int64_t)a.cu_new[a.n_seqs], a.n_tokens)) return;
+    const int n = min(a.part_n[row], a.splits);
+    if (n <= 1) return;
+    const int64_t part = row * a.splits;
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += 32) top = fmaxf(top, a.part_ml[part + s].x);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+        const float2 ml = a.part_ml[part + s];
+        const float f = pow2(ml.x - ref);
+        l += f * ml.y;
+        if (lane * 4 < D) {
+            const float4 o = *(reinterpret_cast<const float4 *>(a.part_o + (part + s) * D) + lane);
+            acc.x += f * o.x, acc.y += f * o.y, acc.z += f * o.z, acc.w += f * o.w;
         }
     }
+    const float inv = paged_inverse(l);
+    if (lane * 4 < D)
+        *reinterpret_cast<uint2 *>((T *)a.out + tok * a.out_stride + (row - tok * a.n_heads) * D + lane * 4) =
+            make_uint2(pack2(acc.x * inv, acc.y * inv, T()), pack2(acc.z * inv, acc.w * inv, T()));
 }
 
 // ---------------------------------------------------------------------------
@@ -634,6 +666,10 @@ static cudaError_t launch_chunk(const PagedAttnArgs &a, cudaStream_t st) {
     const int64_t tiles = a.n_tokens / (2 * tile_tok) + a.n_seqs;
     const dim3 grid((unsigned)tiles, (unsigned)a.cache.n_kv_heads, (unsigned)a.splits);
     k_paged_attn_chunk<T, DP><<<grid, kThreads, ChunkCfg<DP>::SMEM, st>>>(a, q, k, v);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || a.splits == 1) return e;
+    const int64_t rows = a.n_tokens * a.n_heads;
+    k_paged_join<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 

@@ -57,6 +57,30 @@ bool capturing(cudaStream_t st) {
     return s != cudaStreamCaptureStatusNone;
 }
 
+// Pieces of the key axis for the chunk kernel: the number that gives the
+// shortest time of whole rounds of 148 blocks, a block's start and end costing
+// about 3 of its steps of 128 keys (7000 + 3000 clocks against 4000) and the
+// join as much again.
+int chunk_pieces(int64_t blocks, int64_t keys) {
+    const int64_t most = std::min<int64_t>((keys + 255) / 256, 64);
+    int best = 1;
+    int64_t best_cost = INT64_MAX;
+    for (int64_t s = 1; s <= most; ++s) {
+        const int64_t steps = (keys + 128 * s - 1) / (128 * s);
+        const int64_t cost = (blocks * s + 147) / 148 * (steps + 3) + (s > 1 ? 3 : 0);
+        if (cost < best_cost) best = (int)s, best_cost = cost;
+    }
+    return best;
+}
+
+// For the row kernel: about two blocks for each of the two places on an SM,
+// 256 keys or more each. Measured on B200 at 296, 592, 1184, 2368 blocks:
+// 64 requests of 17-4099 keys 122, 108, 106, 113 us; 7 of 30011-65000 keys
+// 232, 231, 246, 241 us.
+int row_pieces(int64_t blocks, int64_t keys) {
+    return (int)std::min<int64_t>(std::min((592 + blocks - 1) / blocks, (keys + 255) / 256), 256);
+}
+
 }  // namespace
 
 extern "C" {
@@ -169,17 +193,15 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         a.part_o = nullptr;
         a.part_ml = nullptr;
         a.count = nullptr;
+        a.part_n = nullptr;
         a.err = (int *)ctx->d_err.p;
-        // pieces of the key axis: enough blocks for about four rounds of the
-        // row kernel's two blocks on each of 148 SMs (the chunk kernel: two
-        // rounds of its one), 256 keys or more each
+        // pieces of the key axis, from the largest lengths that the caller names
         const int64_t rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
         const int64_t blocks = std::min(plan.tiles, n_seqs * ((rows + plan.unit - 1) / plan.unit)) * a.cache.n_kv_heads;
         int64_t keys = std::max(max_len, 1);
         if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + plan.unit / group + 16);
-        const int64_t want = plan.chunk ? 296 : 1184, step = plan.chunk ? 128 : 64;
-        const int64_t splits = std::min((want + blocks - 1) / blocks, (keys + 255) / 256);
-        a.splits = capturing(st) ? 1 : (int)std::min<int64_t>(splits, 256);
+        a.splits = capturing(st) ? 1 : plan.chunk ? chunk_pieces(blocks, keys) : row_pieces(blocks, keys);
+        const int64_t step = plan.chunk ? 128 : 64;
         a.split_keys = (int)(((keys + a.splits - 1) / a.splits + step - 1) / step * step);
         if (a.splits == 1) {
             check_cuda(paged_attn(plan, a, st), "paged attention launch");
@@ -190,15 +212,19 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         const size_t parts = (size_t)n_tokens * n_heads * a.splits;
         a.part_o = ctx->buf("paged_part_o", parts * a.cache.head_dim);
         a.part_ml = (float2 *)ctx->buf("paged_part_ml", parts * 2);
-        DevBuf &count = ctx->ws["paged_count"];
-        const size_t count_bytes = (size_t)plan.tiles * a.cache.n_kv_heads * sizeof(unsigned);
-        if (count.bytes < count_bytes) {
-            count.ensure(count_bytes);
-            check_cuda(cudaMemsetAsync(count.p, 0, count.bytes, st), "clear the piece counters");
+        if (plan.chunk) {
+            a.part_n = (int *)ctx->buf("paged_part_n", (size_t)n_tokens * n_heads);
+        } else {
+            DevBuf &count = ctx->ws["paged_count"];
+            const size_t count_bytes = (size_t)plan.tiles * a.cache.n_kv_heads * sizeof(unsigned);
+            if (count.bytes < count_bytes) {
+                count.ensure(count_bytes);
+                check_cuda(cudaMemsetAsync(count.p, 0, count.bytes, st), "clear the piece counters");
+            }
+            a.count = (unsigned *)count.p;
         }
-        a.count = (unsigned *)count.p;
         check_cuda(paged_attn(plan, a, st), "paged attention launch");
-        ++ctx->n_launches;
+        ctx->n_launches += plan.chunk ? 2 : 1;
         return KK_OK;
     });
 }
