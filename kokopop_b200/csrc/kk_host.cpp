@@ -2027,6 +2027,8 @@ void check_device_error(kk_ctx *ctx) {
                                               std::to_string(e) + ")");
     if (e == kErrPagedWait)
         throw KKError(KK_ERROR_INFERENCE, "paged attention timed out waiting (code " + std::to_string(e) + ")");
+    if (e == kErrQ4Wait)
+        throw KKError(KK_ERROR_INFERENCE, "4-bit product timed out waiting (code " + std::to_string(e) + ")");
     throw KKError(KK_ERROR_INFERENCE, "tensor-core convolution timed out waiting (code " + std::to_string(e) + ")");
 }
 

@@ -439,7 +439,10 @@ struct Q4MatvecArgs {
     const float *bias;  // may be null
     void *out;
     int64_t out_stride;
+    int *err;  // device error word
 };
+// A wait of the 4-bit product for its weights ran out (2 s).
+constexpr int kErrQ4Wait = 79;
 cudaError_t q4_matvec(const Q4MatvecArgs &a, cudaStream_t st);
 
 }  // namespace kk

@@ -5,18 +5,32 @@
 // q - 8 fits the 16-bit types, and a 32-bit x is split into three bfloat16
 // parts (8 + 8 + 8 significant bits, its whole range).
 //
-// The weights are read once, n_out n_in / 2 bytes, and bound it. A warp takes
-// 16 outputs as the M side of mma.sync.m16n8k16 and up to 8 rows of x as its
-// N side, so a row more costs no further work on the weights. The order of k
+// The weights are read once, n_out n_in / 2 bytes, and bound it, with the
+// unpacking close behind: 7 integer operations for 8 weights. A warp takes 16
+// outputs as the M side of mma.sync.m16n8k16 and 8 or 16 rows of x as its N
+// side, so a row more costs no further work on the weights. The order of k
 // within a product is free as long as both sides agree: a lane takes 8
 // consecutive k (one 32-bit word of weights, whose nibbles i and i + 4 are
 // the two halves of one masked word), so nothing is moved between lanes. The
 // products of one group are summed by the tensor cores, then scaled once per
-// output in 32 bits. The warps of a block share the k axis and are joined in
-// shared memory, in the order of the warps.
+// output in 32 bits.
+//
+// The weights come as tensor copies of 256 k (128 bytes, swizzled, so that the
+// words of 8 rows lie in different banks) into a ring of each warp, one lane
+// issuing. x is brought to shared memory a chunk of k at a time by the whole
+// block, split and ordered as the lanes read it, 16 bytes each without a bank
+// twice. The 8 warps of a block lie along the outputs (WR) and along k; the
+// latter are joined in shared memory, in the order of the warps.
 #include "../../include/kokopop_b200.h"
 #include "kk_common.cuh"
 #include "kk_kernels.h"
+#include "kk_ptx.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
+#include <type_traits>
 
 namespace kk {
 
@@ -42,19 +56,45 @@ __device__ __forceinline__ void mma_q4<__nv_bfloat16>(float (&c)[4], const uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// nibbles i and i + 4 of w (i = 0 after the shift) as a pair of values q - 8:
-// placed in the mantissa of 1024 (half) or 128 (bfloat16), whose last place
-// is 1, and 1024 + 8 or 128 + 8 subtracted, exactly
-__device__ __forceinline__ uint32_t pair_of(uint32_t w, __half) {
-    const uint32_t u = (w & 0x000f000fu) | 0x64006400u, b = 0x64086408u;
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
+// The same from a sum of 0.
+template <typename T>
+__device__ __forceinline__ void mma_q4_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    c[0] = c[1] = c[2] = c[3] = 0.f;
+    mma_q4<T>(c, a, b0, b1);
 }
-__device__ __forceinline__ uint32_t pair_of(uint32_t w, __nv_bfloat16) {
-    const uint32_t u = (w & 0x000f000fu) | 0x43004300u, b = 0x43084308u;
-    const __nv_bfloat162 r =
-        __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
+
+// The 8 weights of a word as 4 pairs (nibbles i and i + 4) of values q - 8.
+// The nibbles are placed in the mantissa of 128 (bfloat16) or 1024 (half),
+// whose last place is 1, and 128 + 8 or 1024 + 8 is subtracted by a fused
+// multiply-add; half has room for them 4 places up too, as 1024 + 16 q. All of
+// it is exact.
+__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));  // (w & mask) | bits
+    return r;
+}
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c, __half) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c, __nv_bfloat16) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&v)[4], __half t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t u = w >> (8 * i);
+        v[2 * i] = fma2(mask_or(u, 0x000f000fu, 0x64006400u), 0x3c003c00u, 0xe408e408u, t);      // 1, -1032
+        v[2 * i + 1] = fma2(mask_or(u, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u, t);  // 1 / 16, -72
+    }
+}
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&v)[4], __nv_bfloat16 t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = fma2(mask_or(w >> (4 * i), 0x000f000fu, 0x43004300u), 0x3f803f80u, 0xc308c308u, t);  // 1, -136
 }
 
 // The type multiplied for x of type T, and the parts of one value.
@@ -102,77 +142,284 @@ __device__ __forceinline__ void put(float v, __nv_bfloat16 *p) { *p = __float2bf
 
 }  // namespace
 
-template <typename T>
-__global__ void __launch_bounds__(kQ4Warps * 32) k_q4_matvec(Q4MatvecArgs a) {
+// One block of 256 k of 16 outputs: c = the sum over a group of PG x 32 k,
+// then acc += scale c. at: the lane's word of row gid in the first 16 bytes
+// of the block, w8 its row; x: the lane's 16 bytes of the first 32 k for each
+// tile of rows, x_group and x_part bytes further for the next 32 k and the
+// next part (0 where the lane's row does not exist: it then stays on 16 bytes
+// of zeros); fa: the scales of outputs gid and gid + 8.
+template <typename M, int NB, int PARTS, int PG>
+__device__ __forceinline__ void q4_block(uint32_t at, uint32_t w8, const uint32_t (&x0)[NB],
+                                         const uint32_t (&x_group)[NB], const uint32_t (&x_part)[NB],
+                                         const float (&fa)[2][8 / PG], float (&acc)[NB][4]) {
+    float c[NB][4];
+    uint32_t x[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) x[b] = x0[b];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+        uint32_t v[NB][PARTS][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v[b][p][0]), "=r"(v[b][p][1]), "=r"(v[b][p][2]), "=r"(v[b][p][3])
+                             : "r"(x[b] + p * x_part[b])
+                             : "memory");
+            x[b] += x_group[b];
+        }
+        const uint32_t w = at + ((g * 16) ^ w8);
+        uint32_t ua, ub, fu[4], fv[4];
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(ua) : "r"(w) : "memory");
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(ub) : "r"(w + 1024) : "memory");
+        unpack(ua, fu, M());
+        unpack(ub, fv, M());
+        const uint32_t lo[4] = {fu[0], fv[0], fu[1], fv[1]}, hi[4] = {fu[2], fv[2], fu[3], fv[3]};
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int p = PARTS - 1; p >= 0; --p) {
+                if (g % PG == 0 && p == PARTS - 1)
+                    mma_q4_first<M>(c[b], lo, v[b][p][0], v[b][p][1]);
+                else
+                    mma_q4<M>(c[b], lo, v[b][p][0], v[b][p][1]);
+                mma_q4<M>(c[b], hi, v[b][p][2], v[b][p][3]);
+            }
+        if (g % PG == PG - 1)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[b][e] = fmaf(fa[e >> 1][g / PG], c[b][e], acc[b][e]);
+    }
+}
+
+// WR warps along the outputs, 16 each, the others along k; NB tiles of 8 rows
+// of x.
+template <typename T, int NB, int WR>
+struct Q4Cfg {
+    static constexpr int WK = kQ4Warps / WR;
+    static constexpr int ROWS = 16 * WR;
+    static constexpr int STAGES = 3;
+    static constexpr int TILE = 16 * 128;                              // a block of 256 k
+    static constexpr int CTAS = NB == 1 ? 3 : 2;                       // of an SM
+    static constexpr int X_BYTES = (NB == 1 ? 24 : 48) * 1024;         // of x at a time
+    static constexpr int SMEM = kQ4Warps * STAGES * TILE + X_BYTES + 1024 /*align*/;
+};
+
+template <typename T, int NB, int WR>
+__global__ void __launch_bounds__(kQ4Warps * 32, (Q4Cfg<T, NB, WR>::CTAS))
+    k_q4_matvec(const __grid_constant__ Q4MatvecArgs a, const __grid_constant__ CUtensorMap map_w) {
+    using C = Q4Cfg<T, NB, WR>;
     using M = typename XType<T>::M;
     constexpr int PARTS = XType<T>::PARTS;
-    __shared__ float join[kQ4Warps][16][8];
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *sX = smem + kQ4Warps * C::STAGES * C::TILE;
+    __shared__ __align__(8) uint64_t bar_s[kQ4Warps][C::STAGES];
+    __shared__ __align__(16) uint4 zero_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
-    const int n0 = blockIdx.x * 16;
-    const int64_t r0 = (int64_t)blockIdx.y * 8;
-    const int64_t kb = a.n_in / 2;
-    const int groups = a.n_in / a.group;
-    // outputs past the last read the last row's weights and are not written
-    const int na = min(n0 + gid, a.n_out - 1), nb = min(n0 + gid + 8, a.n_out - 1);
-    const uint8_t *wa = a.w + na * kb + tig * 4, *wb = a.w + nb * kb + tig * 4;
-    const __half *sa = a.scales + (int64_t)na * groups, *sb = a.scales + (int64_t)nb * groups;
-    const bool has_x = r0 + gid < a.n_rows;
-    const T *x = (const T *)a.x + (has_x ? r0 + gid : 0) * a.x_stride + tig * 8;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int steps = a.group / 32;
-    for (int g = warp; g < groups; g += kQ4Warps) {
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < steps; ++s) {
-            const int64_t k = (int64_t)g * a.group + s * 32;
-            const uint32_t ua = *reinterpret_cast<const uint32_t *>(wa + k / 2);
-            const uint32_t ub = *reinterpret_cast<const uint32_t *>(wb + k / 2);
-            uint32_t b[PARTS][4];
-            if (has_x) {
-                load_x(x + k, b);
-            } else {
+    const int wr = warp / C::WK, wk = warp % C::WK;
+    const int n0 = blockIdx.x * C::ROWS + wr * 16;
+    const int64_t r0 = (int64_t)blockIdx.y * (8 * NB);
+    const int shift = 31 - __clz(a.group), groups = a.n_in >> shift, blocks = (a.n_in + 255) / 256;
+    const int rows = (int)min(a.n_rows - r0, (int64_t)(8 * NB));
+    const uint32_t ring = smem_u32(smem + warp * C::STAGES * C::TILE), bars = smem_u32(bar_s[warp]);
+    if (lane == 0) {
+        for (int i = 0; i < C::STAGES; ++i) mbar_init(bars + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // the warp's first blocks of 256 k: wk, wk + WK, ...
+        for (int i = 0; i < C::STAGES - 1; ++i)
+            if (wk + i * C::WK < blocks) {
+                mbar_expect_tx(bars + 8 * i, C::TILE);
+                tma_load_2d(ring + i * C::TILE, &map_w, bars + 8 * i, (wk + i * C::WK) * 128, n0);
+            }
+    }
+    __syncwarp();
+
+    // scales of this lane's outputs; outputs past the last are not written
+    const __half *sa = a.scales + (int64_t)min(n0 + gid, a.n_out - 1) * groups;
+    const __half *sb = a.scales + (int64_t)min(n0 + 8 + gid, a.n_out - 1) * groups;
+    // the lane's word in row gid of a block; its 16-byte chunk is XORed by the row
+    const uint32_t at0 = ring + gid * 128 + tig * 4;
+    float acc[NB][4];
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) b[p][0] = b[p][1] = b[p][2] = b[p][3] = 0u;
+    for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.f;
+
+    // x in shared memory: [group of 32 k][part][row][8 k of lane tig]; 16
+    // bytes of zeros for the rows that do not exist
+    const uint32_t part = rows * 64, step = part * PARTS;
+    const int chunk = min(C::X_BYTES / (int)step / 8 * 256, blocks * 256);
+    if (tid == 0) zero_s = make_uint4(0u, 0u, 0u, 0u);
+    uint32_t x_at[NB], x_group[NB], x_part[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int r = 8 * b + gid;
+        x_at[b] = r < rows ? smem_u32(sX) + r * 64 + tig * 16 : smem_u32(&zero_s);
+        x_group[b] = r < rows ? step : 0;
+        x_part[b] = r < rows ? part : 0;
+    }
+
+    bool ok = true;
+    int blk = wk;
+    uint32_t st = 0, phase = 0;  // stage and phase of the warp's block
+    for (int c0 = 0; c0 < a.n_in; c0 += chunk) {
+        const int c1 = min(c0 + chunk, a.n_in);
+        // x of [c0, c1), 8 values of a row at a time and 0 up to the next
+        // multiple of 256: the weights there read as 0, which stands for -8
+        if (c0 > 0) __syncthreads();
+        const int per_row = (c1 - c0 + 255) / 256 * 32, items = rows * per_row;
+        const uint32_t inv = 0xffffffffu / per_row + 1;  // item / per_row, items are below 2^16
+        constexpr int BATCH = 4;  // loads in flight of a thread
+        for (int it = tid; it < items; it += BATCH * kQ4Warps * 32) {
+            uint32_t v[BATCH][PARTS][4];
+            int r[BATCH], k8[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int at = it + j * kQ4Warps * 32;
+                r[j] = (int)__umulhi((uint32_t)at, inv);
+                k8[j] = at - r[j] * per_row;
+                if (at < items && c0 + k8[j] * 8 < c1) {
+                    load_x((const T *)a.x + (r0 + r[j]) * a.x_stride + c0 + k8[j] * 8, v[j]);
+                } else {
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) v[j][p][0] = v[j][p][1] = v[j][p][2] = v[j][p][3] = 0u;
+                }
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t f[4] = {pair_of(ua >> (8 * h), M()), pair_of(ub >> (8 * h), M()),
-                                       pair_of(ua >> (8 * h + 4), M()), pair_of(ub >> (8 * h + 4), M())};
+            for (int j = 0; j < BATCH; ++j) {
+                if (it + j * kQ4Warps * 32 >= items) break;
+                uint8_t *to = sX + (k8[j] >> 2) * step + r[j] * 64 + (k8[j] & 3) * 16;
 #pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p) mma_q4<M>(c, f, b[p][2 * h], b[p][2 * h + 1]);
+                for (int p = 0; p < PARTS; ++p)
+                    *reinterpret_cast<uint4 *>(to + p * part) =
+                        make_uint4(v[j][p][0], v[j][p][1], v[j][p][2], v[j][p][3]);
             }
         }
-        const float s0 = __half2float(sa[g]), s1 = __half2float(sb[g]);
-        acc[0] = fmaf(s0, c[0], acc[0]);
-        acc[1] = fmaf(s0, c[1], acc[1]);
-        acc[2] = fmaf(s1, c[2], acc[2]);
-        acc[3] = fmaf(s1, c[3], acc[3]);
+        __syncthreads();
+        for (; ok && blk * 256 < c1; blk += C::WK) {
+            const uint32_t bar = bars + 8 * st, at = at0 + st * C::TILE;
+            const int next = blk + (C::STAGES - 1) * C::WK;
+            if (lane == 0 && next < blocks) {
+                const uint32_t to = st == 0 ? C::STAGES - 1 : st - 1;
+                mbar_expect_tx(bars + 8 * to, C::TILE);
+                tma_load_2d(ring + to * C::TILE, &map_w, bars + 8 * to, next * 128, n0);
+            }
+            uint32_t x[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) x[b] = x_at[b] + ((blk * 256 - c0) >> 5) * x_group[b];
+            auto run = [&](auto pg) {
+                constexpr int PG = decltype(pg)::value, NS = 8 / PG;
+                // the block's scales: loaded before its weights are waited for
+                float fa[2][NS];
+                const int s0 = blk * NS;
+#pragma unroll
+                for (int g = 0; g < NS; ++g) {
+                    fa[0][g] = s0 + g < groups ? __half2float(__ldg(sa + s0 + g)) : 0.f;
+                    fa[1][g] = s0 + g < groups ? __half2float(__ldg(sb + s0 + g)) : 0.f;
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait_tight(bar, phase, a.err, kErrQ4Wait));
+                if (ok) q4_block<M, NB, PARTS, PG>(at, gid * 16, x, x_group, x_part, fa, acc);
+            };
+            if (shift == 5)
+                run(std::integral_constant<int, 1>());
+            else if (shift == 6)
+                run(std::integral_constant<int, 2>());
+            else
+                run(std::integral_constant<int, 4>());
+            if (!ok) break;
+            __syncwarp();  // the stage is read before its next copy is issued
+            st = st + 1 == C::STAGES ? (phase ^= 1, 0) : st + 1;
+        }
     }
-    join[warp][gid][tig * 2] = acc[0];
-    join[warp][gid][tig * 2 + 1] = acc[1];
-    join[warp][gid + 8][tig * 2] = acc[2];
-    join[warp][gid + 8][tig * 2 + 1] = acc[3];
+    if (!ok)  // copies in flight land before the block ends
+        for (int j = 0; j < C::STAGES && blk + j * C::WK < blocks; ++j) {
+            mbar_wait(bars + 8 * st, phase, a.err, kErrQ4Wait, TC_DRAIN_NS);
+            st = st + 1 == C::STAGES ? (phase ^= 1, 0) : st + 1;
+        }
     __syncthreads();
-    if (tid < 128) {
-        const int n = n0 + (tid & 15), r = tid >> 4;
-        if (n < a.n_out && r0 + r < a.n_rows) {
+    // join: [wk][output][row]
+    float *join = reinterpret_cast<float *>(smem);
+    constexpr int COLS = 8 * NB, LEN = C::ROWS * COLS;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            join[wk * LEN + (wr * 16 + 8 * (e >> 1) + gid) * COLS + 8 * b + 2 * tig + (e & 1)] = acc[b][e];
+    __syncthreads();
+    for (int it = tid; it < LEN; it += kQ4Warps * 32) {
+        const int n = blockIdx.x * C::ROWS + it % C::ROWS, r = it / C::ROWS;
+        if (n < a.n_out && r < rows) {
             float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < kQ4Warps; ++w) v += join[w][tid & 15][r];
+            for (int w = 0; w < C::WK; ++w) v += join[w * LEN + it % C::ROWS * COLS + r];
             if (a.bias) v += a.bias[n];
             put(v, (T *)a.out + (r0 + r) * a.out_stride + n);
         }
     }
 }
 
-cudaError_t q4_matvec(const Q4MatvecArgs &a, cudaStream_t st) {
-    const dim3 grid((unsigned)((a.n_out + 15) / 16), (unsigned)((a.n_rows + 7) / 8));
-    if (a.dtype == KK_DTYPE_F32)
-        k_q4_matvec<float><<<grid, kQ4Warps * 32, 0, st>>>(a);
-    else if (a.dtype == KK_DTYPE_F16)
-        k_q4_matvec<__half><<<grid, kQ4Warps * 32, 0, st>>>(a);
-    else
-        k_q4_matvec<__nv_bfloat16><<<grid, kQ4Warps * 32, 0, st>>>(a);
+static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> g_encode{nullptr};
+
+// the weights as bytes, boxes of 128 bytes x 16 outputs, swizzled; outside reads as 0
+static cudaError_t weight_map(const Q4MatvecArgs &a, CUtensorMap *m) {
+    auto encode = g_encode.load(std::memory_order_acquire);
+    if (!encode) {
+        cudaDriverEntryPointQueryResult q;
+        void *fn = nullptr;
+        cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q);
+        if (e != cudaSuccess) return e;
+        if (q != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
+        encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+        g_encode.store(encode, std::memory_order_release);
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)a.n_in / 2, (cuuint64_t)a.n_out};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.n_in / 2};
+    const cuuint32_t box[2] = {128, 16}, step[2] = {1, 1};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)a.w, dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+template <typename T, int NB, int WR>
+static cudaError_t launch_q4(const Q4MatvecArgs &a, cudaStream_t st) {
+    using C = Q4Cfg<T, NB, WR>;
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(k_q4_matvec<T, NB, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return e;
+        done[dev].store(true, std::memory_order_release);
+    }
+    CUtensorMap m;
+    e = weight_map(a, &m);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)((a.n_out + C::ROWS - 1) / C::ROWS), (unsigned)((a.n_rows + 8 * NB - 1) / (8 * NB)));
+    k_q4_matvec<T, NB, WR><<<grid, kQ4Warps * 32, C::SMEM, st>>>(a, m);
     return cudaGetLastError();
+}
+
+template <typename T, int NB>
+static cudaError_t launch_q4_rows(const Q4MatvecArgs &a, cudaStream_t st) {
+    if (a.n_out >= 16384) return launch_q4<T, NB, 4>(a, st);
+    if (a.n_out >= 32 * 148) return launch_q4<T, NB, 2>(a, st);
+    return launch_q4<T, NB, 1>(a, st);
+}
+
+template <typename T>
+static cudaError_t launch_q4_of(const Q4MatvecArgs &a, cudaStream_t st) {
+    return a.n_rows <= 8 ? launch_q4_rows<T, 1>(a, st) : launch_q4_rows<T, 2>(a, st);
+}
+
+cudaError_t q4_matvec(const Q4MatvecArgs &a, cudaStream_t st) {
+    if (a.dtype == KK_DTYPE_F32) return launch_q4_of<float>(a, st);
+    if (a.dtype == KK_DTYPE_F16) return launch_q4_of<__half>(a, st);
+    return launch_q4_of<__nv_bfloat16>(a, st);
 }
 
 }  // namespace kk

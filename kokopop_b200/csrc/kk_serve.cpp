@@ -261,6 +261,7 @@ int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in
         a.bias = bias;
         a.out = out;
         a.out_stride = out_stride;
+        a.err = (int *)ctx->d_err.p;
         check_cuda(q4_matvec(a, stream_of(ctx, stream)), "4-bit product launch");
         ++ctx->n_launches;
         return KK_OK;
