@@ -19,8 +19,8 @@ namespace kk {
 // All of it is integer work on 12 bytes written per new token, so what counts
 // is that it is one launch without a workspace: every block scans the lengths
 // itself (kPtChunk requests at a time, so that any number of requests
-// passes), then writes its share of the tokens, each of which finds its
-// request by bisection of the scanned offsets in shared memory. The token at
+// passes), then writes its share of the tokens, 32 of a warp, which find their
+// requests by searching the scanned offsets in shared memory. The token at
 // the start of a new page writes the table entry, so no block reads what
 // another writes.
 // ---------------------------------------------------------------------------
@@ -30,12 +30,32 @@ constexpr int kPtChunk = kPtThreads * kPtPer;
 
 __device__ __forceinline__ int clamp_i32(int64_t v) { return v > INT32_MAX ? INT32_MAX : (int)v; }
 
+// pages of n tokens
+__device__ __forceinline__ int64_t pages_of(int64_t n, int64_t P, int size_bits) {
+    return size_bits >= 0 ? (n + P - 1) >> size_bits : (n + P - 1) / P;
+}
+
+// The last of the n ascending offsets cu that is at most t (cu[0] is), for a
+// whole warp, 32 candidates a round.
+__device__ __forceinline__ int last_at_or_before(const int *cu, int n, int64_t t, int lane) {
+    int x = 0;
+    while (n > 1) {
+        const int step = (n + 31) / 32, i = lane * step;
+        const uint32_t before = __ballot_sync(0xffffffffu, i < n && cu[x + i] <= t);
+        const int k = before ? 31 - __clz(before) : 0;
+        x += k * step;
+        n = min(step, n - k * step);
+    }
+    return x;
+}
+
 __global__ void __launch_bounds__(kPtThreads) k_page_tables(PageTablesArgs a) {
     __shared__ int cu_s[kPtChunk + 1];     // first token of each request of the chunk
     __shared__ int first_s[kPtChunk];      // first new page of each request
     __shared__ int64_t wsum[2][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t P = a.page_size;
+    const int size_bits = (a.page_size & (a.page_size - 1)) == 0 ? 31 - __clz(a.page_size) : -1;
     const int64_t t_per = (a.n_tokens + gridDim.x - 1) / gridDim.x;
     const int64_t t0 = blockIdx.x * t_per, t1 = t0 + t_per < a.n_tokens ? t0 + t_per : a.n_tokens;
     const bool writer = blockIdx.x == gridDim.x - 1;
@@ -50,8 +70,8 @@ __global__ void __launch_bounds__(kPtThreads) k_page_tables(PageTablesArgs a) {
             if (r < a.n_seqs) {
                 const int64_t c = max(a.ctx_len[r], 0);
                 m[j] = max(a.new_len[r], 0);
-                const int64_t old = (c + P - 1) / P;
-                need[j] = max(min((c + m[j] + P - 1) / P, (int64_t)a.max_pages) - old, (int64_t)0);
+                const int64_t old = pages_of(c, P, size_bits);
+                need[j] = max(min(pages_of(c + m[j], P, size_bits), (int64_t)a.max_pages) - old, (int64_t)0);
                 if (writer) a.seq_len[r] = clamp_i32(c + m[j]);
             }
             st += m[j];
@@ -66,13 +86,17 @@ __global__ void __launch_bounds__(kPtThreads) k_page_tables(PageTablesArgs a) {
         }
         if (lane == 31) wsum[0][warp] = it, wsum[1][warp] = ip;
         __syncthreads();
-        int64_t before_t = base_t, before_p = base_p, all_t = base_t, all_p = base_p;
-        for (int w = 0; w < kPtThreads / 32; ++w) {
-            if (w < warp) before_t += wsum[0][w], before_p += wsum[1][w];
-            all_t += wsum[0][w];
-            all_p += wsum[1][w];
+        // every warp sums the 32 warps' totals
+        int64_t wt = wsum[0][lane], wp = wsum[1][lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, wt, o), y = __shfl_up_sync(0xffffffffu, wp, o);
+            if (lane >= o) wt += x, wp += y;
         }
-        int64_t tt = before_t + it - st, pp = before_p + ip - sp;
+        const int64_t all_t = base_t + __shfl_sync(0xffffffffu, wt, 31), all_p = base_p + __shfl_sync(0xffffffffu, wp, 31);
+        const int64_t prev_t = __shfl_sync(0xffffffffu, wt, (warp + 31) & 31),
+                      prev_p = __shfl_sync(0xffffffffu, wp, (warp + 31) & 31);
+        int64_t tt = base_t + (warp > 0 ? prev_t : 0) + it - st, pp = base_p + (warp > 0 ? prev_p : 0) + ip - sp;
 #pragma unroll
         for (int j = 0; j < kPtPer; ++j) {
             const int i = tid * kPtPer + j;
@@ -85,9 +109,18 @@ __global__ void __launch_bounds__(kPtThreads) k_page_tables(PageTablesArgs a) {
         if (tid == 0) cu_s[kPtChunk] = clamp_i32(all_t);
         __syncthreads();
         const int n = min(kPtChunk, a.n_seqs - r0);
-        const int64_t lo = max(t0, base_t), hi = min(t1, all_t);
-        for (int64_t t = lo + tid; t < hi; t += kPtThreads) {
-            int x = 0, y = n - 1;  // the last request that starts at or before t
+        // a warp takes a run of tokens, 32 at a time: their requests lie between
+        // that of the first and that of the last, mostly the same one
+        const int64_t lo = max(t0, base_t), hi_all = min(t1, all_t);
+        const int64_t run = (max(hi_all - lo, (int64_t)0) + kPtThreads - 1) / kPtThreads * 32;
+        const int64_t hi = min(lo + (warp + 1) * run, hi_all);
+        int first = -1;
+        for (int64_t tw = lo + warp * run; tw < hi; tw += 32) {
+            const int64_t t = tw + lane, last = min(tw + 31, hi - 1);
+            if (first < 0 || (first + 1 < n && cu_s[first + 1] <= tw)) first = last_at_or_before(cu_s, n, tw, lane);
+            int x = first, y = first;
+            if (first + 1 < n && cu_s[first + 1] <= last) y = last_at_or_before(cu_s, n, last, lane);
+            if (t >= hi) continue;
             while (x < y) {
                 const int mid = (x + y + 1) >> 1;
                 if (cu_s[mid] <= t)
@@ -96,10 +129,12 @@ __global__ void __launch_bounds__(kPtThreads) k_page_tables(PageTablesArgs a) {
                     y = mid - 1;
             }
             const int r = r0 + x;
-            const int64_t c = max(a.ctx_len[r], 0), pos = c + (t - cu_s[x]);
-            const int64_t old = (c + P - 1) / P, col = pos / P, off = pos - col * P;
+            // positions are below 2^32: two lengths of 31 bits
+            const uint32_t c = (uint32_t)max(a.ctx_len[r], 0), pos = c + (uint32_t)(t - cu_s[x]), size = a.page_size;
+            const uint32_t col = size_bits >= 0 ? pos >> size_bits : pos / size, off = pos - col * size;
+            const uint32_t whole = size_bits >= 0 ? c >> size_bits : c / size, old = whole + (whole * size != c);
             int page = -1;
-            if (col < a.max_pages) {
+            if (col < (uint32_t)a.max_pages) {
                 int32_t *entry = a.table + (int64_t)r * a.max_pages + col;
                 if (col < old) {
                     page = *entry;

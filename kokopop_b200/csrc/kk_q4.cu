@@ -249,6 +249,9 @@ __global__ void __launch_bounds__(kQ4Warps * 32, (Q4Cfg<T, NB, WR>::CTAS))
     // x in shared memory: [group of 32 k][part][row][8 k of lane tig]; 16
     // bytes of zeros for the rows that do not exist
     const uint32_t part = rows * 64, step = part * PARTS;
+    // a warp brings a row, or a power of two of the warps share it
+    const int row_bits = min(32 - __clz(rows - 1), 3), xk = (warp >> row_bits) * 32 + lane,
+              xk_step = kQ4Warps * 32 >> row_bits;
     const int chunk = min(C::X_BYTES / (int)step / 8 * 256, blocks * 256);
     if (tid == 0) zero_s = make_uint4(0u, 0u, 0u, 0u);
     uint32_t x_at[NB], x_group[NB], x_part[NB];
@@ -268,32 +271,31 @@ __global__ void __launch_bounds__(kQ4Warps * 32, (Q4Cfg<T, NB, WR>::CTAS))
         // x of [c0, c1), 8 values of a row at a time and 0 up to the next
         // multiple of 256: the weights there read as 0, which stands for -8
         if (c0 > 0) __syncthreads();
-        const int per_row = (c1 - c0 + 255) / 256 * 32, items = rows * per_row;
-        const uint32_t inv = 0xffffffffu / per_row + 1;  // item / per_row, items are below 2^16
-        constexpr int BATCH = 4;  // loads in flight of a thread
-        for (int it = tid; it < items; it += BATCH * kQ4Warps * 32) {
-            uint32_t v[BATCH][PARTS][4];
-            int r[BATCH], k8[BATCH];
+        const int per_row = (c1 - c0 + 255) / 256 * 32;
+        constexpr int BATCH = PARTS == 1 ? 6 : 3;  // loads in flight of a thread
+        for (int xr = warp & ((1 << row_bits) - 1); xr < rows; xr += 8) {
+            const T *x = (const T *)a.x + (r0 + xr) * a.x_stride + c0;
+            for (int k8 = xk; k8 < per_row; k8 += BATCH * xk_step) {
+                uint32_t v[BATCH][PARTS][4];
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-                const int at = it + j * kQ4Warps * 32;
-                r[j] = (int)__umulhi((uint32_t)at, inv);
-                k8[j] = at - r[j] * per_row;
-                if (at < items && c0 + k8[j] * 8 < c1) {
-                    load_x((const T *)a.x + (r0 + r[j]) * a.x_stride + c0 + k8[j] * 8, v[j]);
-                } else {
+                for (int j = 0; j < BATCH; ++j) {
+                    const int k = (k8 + j * xk_step) * 8;
+                    if (c0 + k < c1) {
+                        load_x(x + k, v[j]);
+                    } else {
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) v[j][p][0] = v[j][p][1] = v[j][p][2] = v[j][p][3] = 0u;
+                        for (int p = 0; p < PARTS; ++p) v[j][p][0] = v[j][p][1] = v[j][p][2] = v[j][p][3] = 0u;
+                    }
                 }
-            }
+                // xk_step is a multiple of 4: k8 % 4 stays
+                uint8_t *to = sX + (k8 >> 2) * step + xr * 64 + (k8 & 3) * 16;
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-                if (it + j * kQ4Warps * 32 >= items) break;
-                uint8_t *to = sX + (k8[j] >> 2) * step + r[j] * 64 + (k8[j] & 3) * 16;
+                for (int j = 0; j < BATCH; ++j)
+                    if (k8 + j * xk_step < per_row)
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-                    *reinterpret_cast<uint4 *>(to + p * part) =
-                        make_uint4(v[j][p][0], v[j][p][1], v[j][p][2], v[j][p][3]);
+                        for (int p = 0; p < PARTS; ++p)
+                            *reinterpret_cast<uint4 *>(to + j * (xk_step >> 2) * step + p * part) =
+                                make_uint4(v[j][p][0], v[j][p][1], v[j][p][2], v[j][p][3]);
             }
         }
         __syncthreads();
