@@ -41,7 +41,6 @@ namespace {
 
 constexpr int kKeys = 16;   // keys of a warp's step
 constexpr int kWarps = 4;
-constexpr int kStages = 3;
 constexpr int kFewRows = 16;  // query rows up to which a call takes this kernel
 constexpr int kMaxPieces = 256;
 constexpr float kGrow = 8.0f;  // base-2 growth of a maximum that is left alone
@@ -49,9 +48,12 @@ constexpr float kGrow = 8.0f;  // base-2 growth of a maximum that is left alone
 template <int DP, int NB>
 struct RowCfg {
     static constexpr int ROWS = 8 * NB;
+    // steps of a warp's ring: 96 KB a block, or 32 KB, which leaves room for
+    // more blocks (heads of 64, 64 requests: 84 us with three steps, 78 with two)
+    static constexpr int STAGES = DP > 64 ? 3 : 2;
     static constexpr int HALF_BYTES = kKeys * 128;   // 64 dims of a block of keys
     static constexpr int TILE = kKeys * DP * 2;      // K or V of one step
-    static constexpr int RING = kWarps * kStages * 2 * TILE;
+    static constexpr int RING = kWarps * STAGES * 2 * TILE;
     static constexpr int OS = DP + 4;                // row stride of the join: no bank twice
     static constexpr int JOIN = (kWarps * ROWS * (OS + 2) + ROWS * (kMaxPieces + 1)) * 4;
     static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + 1024 /*align*/;
@@ -67,16 +69,18 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+template <int OFF>
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a)
+                 : "r"(a), "n"(OFF)
                  : "memory");
 }
+template <int OFF>
 __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a)
+                 : "r"(a), "n"(OFF)
                  : "memory");
 }
 
@@ -125,8 +129,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     constexpr int CH = DP / 8;       // 16-byte chunks of a key
     extern __shared__ __align__(1024) unsigned char sm_raw[];
     unsigned char *sm = (unsigned char *)(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t bar_s[kWarps][kStages];
-    __shared__ uint32_t seen_s[kWarps][kStages];
+    __shared__ __align__(8) uint64_t bar_s[kWarps][C::STAGES];
+    __shared__ uint32_t seen_s[kWarps][C::STAGES];
     __shared__ unsigned last_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
     const int group = a.n_heads / a.cache.n_kv_heads, kvh = blockIdx.y;
@@ -149,31 +153,36 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int k0 = (int)(kbeg + sp * piece), k1 = (int)min((int64_t)k0 + piece, kend);
 
     // this warp's steps: blocks of kKeys keys, kWarps apart
-    const int n_blocks = (k1 - k0 + kKeys - 1) / kKeys;
-    const int n_steps = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;
-    unsigned char *ring = sm + warp * kStages * 2 * C::TILE;
+    unsigned char *ring = sm + warp * C::STAGES * 2 * C::TILE;
     const uint32_t ring_u = smem_u32(ring), bars = smem_u32(bar_s[warp]);
     const T *kc = (const T *)a.cache.k + kvh * a.cache.head_stride;
     const T *vc = (const T *)a.cache.v + kvh * a.cache.head_stride;
     const int32_t *table = a.table + (int64_t)t.r * a.max_pages;
     if (TMA) {
         if (lane == 0) {
-            for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+            for (int i = 0; i < C::STAGES; ++i) mbar_init(bars + 8 * i, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
     }
 
-    const int box = min(page_size, kKeys), boxes = kKeys / box;  // TMA: tokens of a copy, copies of a block
-    auto issue = [&](int s) {
-        if (s < n_steps) {
-            const int key0 = k0 + (warp + s * kWarps) * kKeys, st = s % kStages;
+    // TMA: the copy of this lane, 64 dims of one box of a page's tokens, of K or V
+    const int boxes = page_size < kKeys ? 2 : 1, box = page_size < kKeys ? 8 : kKeys;
+    const int part = lane & (boxes - 1), half = (lane >> (boxes - 1)) & (HALVES - 1),
+              kv = lane >> (boxes - 1) >> (HALVES - 1);
+    const uint32_t copy_to = ring_u + kv * C::TILE + half * C::HALF_BYTES + part * box * 128;
+    const CUtensorMap *copy_map = kv ? &map_v : &map_k;
+    const int page_bits = (page_size & (page_size - 1)) == 0 ? 31 - __clz(page_size) : -1;
+    auto page_col = [&](int key) { return page_bits >= 0 ? key >> page_bits : key / page_size; };
+    int next_key = k0 + warp * kKeys, next_stage = 0;  // of the next block to copy
+    auto issue = [&] {
+        if (next_key < k1) {
+            const int key0 = next_key, st = next_stage;
             if (TMA) {
-                const int part = lane & (boxes - 1), half = (lane / boxes) % HALVES, v = lane / (boxes * HALVES);
                 const int key = key0 + part * box;
                 int page = -1, off = 0;
-                if (v < 2 && key < k1) {
-                    const int col = key / page_size;
+                if (kv < 2 && key < k1) {
+                    const int col = page_col(key);
                     page = table[col];
                     off = key - col * page_size;
                     if (page < 0 || page >= a.cache.n_pages) page = -1;
@@ -185,15 +194,13 @@ __global__ void __launch_bounds__(kWarps * 32)
                     mbar_expect_tx(bars + 8 * st, 2 * C::TILE);
                 }
                 __syncwarp();
-                if (v < 2)
-                    tma_load_4d(ring_u + (st * 2 + v) * C::TILE + half * C::HALF_BYTES + part * box * 128,
-                                v ? &map_v : &map_k, bars + 8 * st, 64 * half, off, kvh, page);
+                if (kv < 2) tma_load_4d(copy_to + st * 2 * C::TILE, copy_map, bars + 8 * st, 64 * half, off, kvh, page);
             } else {
                 // lane = key: where its row lies
                 int64_t at = -1;
                 const int key = key0 + (lane & (kKeys - 1));
                 if (key < k1 && key >= lo) {
-                    const int col = key / page_size, page = table[col];
+                    const int col = page_col(key), page = table[col];
                     if (page >= 0 && page < a.cache.n_pages)
                         at = page * a.cache.page_stride + (key - col * page_size) * a.cache.token_stride;
                 }
@@ -213,9 +220,11 @@ __global__ void __launch_bounds__(kWarps * 32)
             }
         }
         if (!TMA) cp_commit();
+        next_key += kWarps * kKeys;
+        next_stage = next_stage + 1 == C::STAGES ? 0 : next_stage + 1;
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) issue(s);
+    for (int s = 0; s < C::STAGES - 1; ++s) issue();
 
     // Q^T fragments: columns (rows of Q) gid and, NB 2, gid + 8
     uint32_t qf[KC][NB][2];
@@ -254,24 +263,24 @@ __global__ void __launch_bounds__(kWarps * 32)
     // keys that every row sees need no mask
     const int all_lo = a.window > 0 ? pos_last - a.window + 1 : 0, all_hi = min(pos_first, k1 - 1);
     // lane's part of the fragments: K rows (m) and V rows (k, transposed)
-    const int k_row = (lane & 7) + (lane & 8), k_ch = lane >> 4;
-    const int v_row = (lane & 7) + ((lane >> 4) << 3), v_ch = (lane >> 3) & 1;
+    // their 16-byte chunk is XORed by the row, chunk 2 k + c of a half in two
+    // steps: (c ^ row) 16 here, 2 k 16 where it is read
+    const uint32_t k_at = ((lane & 7) + (lane & 8)) * 128 + ((lane >> 4 ^ lane) & 7) * 16;
+    const uint32_t v_at = ((lane & 7) + (lane >> 4 << 3)) * 128 + ((lane >> 3 & 1 ^ lane) & 7) * 16;
     bool ok = true;
-    int s = 0;
-    for (; s < n_steps; ++s) {
-        issue(s + kStages - 1);
-        const int st = s % kStages;
+    int st = 0, phase = 0, key0 = k0 + warp * kKeys;
+    for (; key0 < k1; key0 += kWarps * kKeys) {
+        issue();
         if (TMA) {
-            ok = mbar_wait_tight(bars + 8 * st, (s / kStages) & 1, a.err, kErrPagedWait);
+            ok = mbar_wait_tight(bars + 8 * st, phase, a.err, kErrPagedWait);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
         } else {
-            cp_wait<kStages - 1>();
+            cp_wait<C::STAGES - 1>();
             __syncwarp();
         }
         const uint32_t kt = ring_u + st * 2 * C::TILE, vt = kt + C::TILE;
         const uint32_t seen = seen_s[warp][st];
-        const int key0 = k0 + (warp + s * kWarps) * kKeys;
         if (TMA && (key0 < lo || key0 + kKeys > k1)) {
             // values of tokens outside the range may be anything, and 0 times
             // a NaN is one: their rows become 0
@@ -293,8 +302,14 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
         for (int k = 0; k < KC; k += 2) {  // two chains of products
             uint32_t f[4], g[4];
-            ldsm4(kt + k / 4 * C::HALF_BYTES + k_row * 128 + ((((2 * k + k_ch) ^ k_row) & 7) * 16), f);
-            ldsm4(kt + k / 4 * C::HALF_BYTES + k_row * 128 + ((((2 * k + 2 + k_ch) ^ k_row) & 7) * 16), g);
+            const uint32_t at = (kt + k_at) ^ (k % 4 * 32), next = (kt + k_at) ^ ((k + 1) % 4 * 32);
+            if (k < 4) {
+                ldsm4<0>(at, f);
+                ldsm4<0>(next, g);
+            } else {
+                ldsm4<C::HALF_BYTES>(at, f);
+                ldsm4<C::HALF_BYTES>(next, g);
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 mma16<T>(sc[b], f, qf[k][b][0], qf[k][b][1]);
@@ -356,16 +371,22 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
             uint32_t f[4];
-            ldsm4t(vt + i / 4 * C::HALF_BYTES + v_row * 128 + ((((2 * i + v_ch) ^ v_row) & 7) * 16), f);
+            if (i < 4)
+                ldsm4t<0>((vt + v_at) ^ (i % 4 * 32), f);
+            else
+                ldsm4t<C::HALF_BYTES>((vt + v_at) ^ (i % 4 * 32), f);
 #pragma unroll
             for (int b = 0; b < NB; ++b) mma16<T>(o[i][b], f, p[b][0], p[b][1]);
         }
         __syncwarp();  // the stage is read before its next copies are issued
+        st = st + 1 == C::STAGES ? (phase ^= 1, 0) : st + 1;
     }
     if (TMA) {
         if (!ok)  // the copies still in flight land before the block ends
-            for (int c = s; c < min(s + kStages, n_steps); ++c)
-                mbar_wait(bars + 8 * (c % kStages), (c / kStages) & 1, a.err, kErrPagedWait, TC_DRAIN_NS);
+            for (; key0 < min(next_key, k1); key0 += kWarps * kKeys) {
+                mbar_wait(bars + 8 * st, phase, a.err, kErrPagedWait, TC_DRAIN_NS);
+                st = st + 1 == C::STAGES ? (phase ^= 1, 0) : st + 1;
+            }
     } else {
         cp_wait<0>();
     }
