@@ -83,6 +83,28 @@ class PagedCache(ctypes.Structure):
                          head_stride)
 
 
+def q4_pack(w: np.ndarray, group: int):
+    """Weights [n_out, n_in] as the 4-bit products take them: bytes [n_out,
+    n_in / 2] and half scales [n_out, n_in / group]. A group's scale is its
+    largest magnitude / 7, a weight the nearest q - 8 with q in [1, 15]."""
+    w = np.asarray(w, np.float32)
+    if w.ndim != 2 or group not in (32, 64, 128) or w.shape[1] % group != 0:
+        raise KKError(KK_ERROR_INVALID_ARGUMENT, "weights must be [n_out, n_in] with n_in a multiple of 32, 64 or 128")
+    g = w.reshape(w.shape[0], -1, group)
+    scales = (np.abs(g).max(axis=2) / 7.0).astype(np.float16)
+    s = scales.astype(np.float32)[..., None]
+    q = np.where(s > 0, np.rint(np.divide(g, s, out=np.zeros_like(g), where=s > 0)), 0.0)
+    q = (np.clip(q, -7, 7) + 8).astype(np.uint8).reshape(w.shape)
+    return q[:, 0::2] | q[:, 1::2] << 4, scales
+
+
+def q4_unpack(q: np.ndarray, scales: np.ndarray, group: int) -> np.ndarray:
+    """The float32 weights that q4_pack's bytes and scales stand for."""
+    v = np.empty((q.shape[0], 2 * q.shape[1]), np.float32)
+    v[:, 0::2], v[:, 1::2] = q & 15, q >> 4
+    return (v - 8.0) * np.repeat(scales.astype(np.float32), group, axis=1)
+
+
 class ProfileRecord(ctypes.Structure):
     _fields_ = [
         ("kind", ctypes.c_int32),

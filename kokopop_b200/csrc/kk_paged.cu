@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(kPtThreads) k_page_tables(PageTablesArgs a) {
             const int64_t x = __shfl_up_sync(0xffffffffu, wt, o), y = __shfl_up_sync(0xffffffffu, wp, o);
             if (lane >= o) wt += x, wp += y;
         }
-        const int64_t all_t = base_t + __shfl_sync(0xffffffffu, wt, 31), all_p = base_p + __shfl_sync(0xffffffffu, wp, 31);
+        const int64_t all_t = base_t + __shfl_sync(0xffffffffu, wt, 31),
+                      all_p = base_p + __shfl_sync(0xffffffffu, wp, 31);
         const int64_t prev_t = __shfl_sync(0xffffffffu, wt, (warp + 31) & 31),
                       prev_p = __shfl_sync(0xffffffffu, wp, (warp + 31) & 31);
         int64_t tt = base_t + (warp > 0 ? prev_t : 0) + it - st, pp = base_p + (warp > 0 ? prev_p : 0) + ip - sp;

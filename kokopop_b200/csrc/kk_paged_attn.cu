@@ -508,7 +508,8 @@ static cudaError_t launch_row(const PagedAttnArgs &a, int64_t tiles, cudaStream_
 template <typename T, int DP>
 static cudaError_t launch_row_of(const PagedAttnPlan &p, const PagedAttnArgs &a, cudaStream_t st) {
     const bool tma = row_by_tensor(a.cache);
-    if (p.unit == 8) return tma ? launch_row<T, DP, 1, true>(a, p.tiles, st) : launch_row<T, DP, 1, false>(a, p.tiles, st);
+    if (p.unit == 8)
+        return tma ? launch_row<T, DP, 1, true>(a, p.tiles, st) : launch_row<T, DP, 1, false>(a, p.tiles, st);
     return tma ? launch_row<T, DP, 2, true>(a, p.tiles, st) : launch_row<T, DP, 2, false>(a, p.tiles, st);
 }
 

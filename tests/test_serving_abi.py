@@ -2,6 +2,7 @@
 call below is right but for one argument."""
 import ctypes
 
+import numpy as np
 import pytest
 
 import kokopop_b200 as kb
@@ -100,3 +101,24 @@ def test_the_cache_structure_has_the_headers_layout():
     c = kb.PagedCache(1, 2, kb.DTYPE_BF16, 3, 4, 5, 8)
     assert ctypes.sizeof(c) == 64
     assert (c.page_stride, c.token_stride, c.head_stride) == (4 * 5 * 8, 40, 8)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_q4_pack_is_the_nearest_of_its_grid(group):
+    rng = np.random.default_rng(group)
+    w = rng.normal(0.0, 1.0, (7, 384)).astype(np.float32)
+    w[2, :group] = 0.0  # a group of zeros has scale 0
+    q, s = kb.q4_pack(w, group)
+    assert q.dtype == np.uint8 and q.shape == (7, 192) and s.dtype == np.float16 and s.shape == (7, 384 // group)
+    assert s[2, 0] == 0.0
+    back = kb.q4_unpack(q, s, group)
+    step = np.repeat(s.astype(np.float32), group, axis=1)
+    # half a step, and what rounding the scale to half takes from the 7 steps of the largest
+    assert (np.abs(back - w) <= step * (0.5 + 7 * 2.0 ** -11) + 1e-6).all()
+    assert back[0, 5] == ((q[0, 2] >> 4) - 8.0) * np.float32(s[0, 0])
+
+
+def test_q4_pack_refuses_other_shapes():
+    for w, group in ((np.zeros(64), 32), (np.zeros((2, 48)), 32), (np.zeros((2, 64)), 16)):
+        with pytest.raises(kb.KKError):
+            kb.q4_pack(w, group)
