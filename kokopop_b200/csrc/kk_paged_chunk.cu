@@ -44,9 +44,9 @@ constexpr int kTile = 128;       // rows of a tile, keys of a step
 constexpr int kStages = 2;       // pairs of a V tile and the next step's K tile
 constexpr int kThreads = 384;
 // registers of a thread: 168 at launch (3 warpgroups), moved from the copy and
-// MMA warpgroup to the two that hold a row of scores: 88 + 2 x 208 = 3 x 168
-constexpr int kRegsFew = 88, kRegsMany = 208;
-constexpr int kMmaWarp = 8, kCopyWarp = 9, kMmaWarp1 = 10;
+// MMA warpgroup to the two that hold a row of scores: 72 + 2 x 216 = 3 x 168
+constexpr int kRegsFew = 72, kRegsMany = 216;
+constexpr int kScoreWarp = 8, kCopyWarp = 9, kValueWarp = 10;
 constexpr float kGrow = 8.0f;    // base-2 growth of a maximum that is left alone
 
 template <int DP>
@@ -54,9 +54,8 @@ struct ChunkCfg {
     static constexpr int TILE_BYTES = kTile * DP * 2;
     static constexpr int HALF_BYTES = kTile * 128;   // 64 dims of a tile
     static constexpr int SMEM = (2 + 2 * kStages) * TILE_BYTES + 1024 /*barriers*/ + 1024 /*align*/;
-    static constexpr bool P_OVER_S = DP > 64;
-    // tensor memory columns
-    static constexpr int S0 = 0, O0 = 2 * kTile, P0 = P_OVER_S ? 0 : O0 + 2 * DP, P_STEP = P_OVER_S ? kTile : kTile / 2;
+    // tensor memory columns: S of either tile in turn, P and O of both
+    static constexpr int S0 = 0, P0 = kTile, O0 = 2 * kTile;
     static constexpr int COLS = 512;
 };
 static_assert(ChunkCfg<128>::SMEM <= 227 * 1024, "shared memory");
@@ -205,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *sQ = smem, *sKV = smem + 2 * C::TILE_BYTES;
     const uint32_t bars = smem_u32(sKV + 2 * kStages * C::TILE_BYTES);
     const uint32_t bQ = bars, bFull = bars + 16, bEmpty = bFull + 8 * kStages, bS = bEmpty + 8 * kStages,
-                   bP = bS + 16, bPV = bP + 32, bDrain = bPV + 16, bZero = bDrain + 16, bTurn = bZero + 8;
+                   bP = bS + 16, bPV = bP + 32, bDrain = bPV + 16, bFree = bDrain + 16;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bQ + 8 * i, 1);
@@ -216,16 +215,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < kStages; ++i) {
             mbar_init(bFull + 8 * i, 1);
-            mbar_init(bEmpty + 8 * i, 2);  // the issuers of both tiles
+            mbar_init(bEmpty + 8 * i, 2);  // both issuers
         }
         mbar_init(bDrain, 1);
         mbar_init(bDrain + 8, 1);
-        mbar_init(bZero, 2);
-        mbar_init(bTurn, 4);      // the softmax warps of a tile
-        mbar_init(bTurn + 8, 4);
+        mbar_init(bFree, 4);  // the softmax warps of the tile whose scores they are
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) {
+    if (warp == kScoreWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
                      "r"(C::COLS)
                      : "memory");
@@ -238,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // The roles part here for good: each side has its own register budget, and
     // they meet once more at the block barrier that frees tensor memory.
-    if (warp >= kMmaWarp) {
+    if (warp >= kScoreWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
         if (warp == kCopyWarp) {
             // Q of both tiles, then pair i = (V of step i - 1, K of step i) into
@@ -291,99 +288,106 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (n_step[x] > 0) mbar_wait(bQ + 8 * x, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
             }
             __syncwarp();
-        } else if (warp == kMmaWarp || warp == kMmaWarp1) {
-            // A warp per tile, so that neither waits for the other's softmax.
-            // The whole warp walks the steps, so that every operand of an MMA
-            // is the same in all lanes and sits in a uniform register; one
+        } else if (warp == kScoreWarp || warp == kValueWarp) {
+            // One warp issues the products with K, the other those with V.
+            // Both walk the steps whole, so that every operand of an MMA is
+            // the same in all lanes and sits in a uniform register; one
             // elected lane issues. (Issued from code of one lane, an MMA of 64
             // clocks cost 75-105 clocks of issue.)
-            constexpr uint32_t id_s = idesc_of(BF16, 0, kTile), id_o = idesc_of(BF16, 1, DP);
-            const int x = __shfl_sync(0xffffffffu, warp == kMmaWarp ? 0 : 1, 0);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
-            const uint32_t q = desc_lo(base + x * C::TILE_BYTES, 16);
-            const uint32_t dv = desc_lo(base + 2 * C::TILE_BYTES, C::HALF_BYTES),
-                           dk = desc_lo(base + 3 * C::TILE_BYTES, 16);
-            const uint32_t tS = tm + C::S0 + x * kTile, tO = tm + C::O0 + x * DP, tP = tm + C::P0 + x * C::P_STEP;
-            const int n = __shfl_sync(0xffffffffu, x ? n_step[1] : n_step[0], 0);
-            const int all = __shfl_sync(0xffffffffu, steps, 0);
+            const int n0 = __shfl_sync(0xffffffffu, n_step[0], 0), n1 = __shfl_sync(0xffffffffu, n_step[1], 0);
+            const int all = max(n0, n1);
             bool ok = true;
-            uint32_t zeroed = 0;
             auto wait = [&](uint32_t bar, uint32_t parity) {
                 ok = __all_sync(0xffffffffu, mbar_wait_tight(bar, parity, a.err, kErrPagedWait));
                 return ok;
             };
-            auto score = [&](uint32_t k, int s) {  // S = Q K^T, K in stage s
-                fence_after_sync();
-                if (elect_one()) {
+            if (warp == kScoreWarp) {
+                constexpr uint32_t id = idesc_of(BF16, 0, kTile);
+                const uint32_t dq = desc_lo(base, 16), dk = desc_lo(base + 3 * C::TILE_BYTES, 16);
+                int turn = 0;  // of the scores' columns
+                for (int j = 0; j < all && ok; ++j) {
+                    const int s = j % kStages;  // K of step j is in pair j
+                    if (!wait(bFull + 8 * s, j / kStages & 1)) break;
+                    const uint32_t k = dk + 2 * s * (C::TILE_BYTES >> 4);
 #pragma unroll
-                    for (int d = 0; d < DP / 16; ++d) {
-                        const uint32_t at = (d / 4 * C::HALF_BYTES + d % 4 * 32) >> 4;
-                        mma_ss(tS, q + at, k + at, id_s, d > 0);
-                    }
-                    mma_commit(bS + 8 * x);
-                    mma_commit(bEmpty + 8 * s);
-                }
-                __syncwarp();
-            };
-            const int r_lo = (int)max(min(lo - k0, (int64_t)kTile), (int64_t)0);  // rows of step 0 below the keys
-            if (all > 0 && wait(bFull, 0)) {
-                if (n > 0) {
-                    if (wait(bQ + 8 * x, 0)) score(dk, 0);
-                } else if (elect_one()) {
-                    mbar_arrive(bEmpty);
-                }
-            }
-            __syncwarp();
-            for (int j = 0; j < all && ok; ++j) {
-                const int s = (j + 1) % kStages;
-                if (!wait(bFull + 8 * s, (j + 1) / kStages & 1)) break;
-                // the rows of V outside the block's keys become 0
-                const int r_hi = (int)min(k1 - k0 - (int64_t)j * kTile, (int64_t)kTile);
-                if ((j == 0 && r_lo > 0) || r_hi < kTile) {
-                    uint8_t *v = sKV + 2 * s * C::TILE_BYTES;
-                    for (int e = lane + 32 * x; e < kTile * HALVES * 8; e += 64) {
-                        const int row = (e >> 3) % kTile, h = e / (kTile * 8);
-                        if ((j == 0 && row < r_lo) || row >= r_hi)
-                            *reinterpret_cast<uint4 *>(v + h * C::HALF_BYTES + row * 128 + (e & 7) * 16) =
-                                make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (elect_one()) mbar_arrive(bZero);  // both issuers' halves, bounded like every wait
-                    if (!wait(bZero, zeroed++ & 1)) break;
-                }
-                if (j >= n) {  // this tile has no such step: only the stage is given back
-                    if (elect_one()) mbar_arrive(bEmpty + 8 * s);
-                    __syncwarp();
-                    continue;
-                }
-                const uint32_t at = 2 * s * (C::TILE_BYTES >> 4);
-                // O += P V, the first 64 keys as soon as their weights are there
+                    for (int x = 0; x < 2; ++x) {
+                        if (j >= (x ? n1 : n0)) continue;
+                        if (j == 0 && !wait(bQ + 8 * x, 0)) break;
+                        // the scores before have been read
+                        if (turn > 0 && !wait(bFree, (turn - 1) & 1)) break;
+                        ++turn;
+                        fence_after_sync();
+                        if (elect_one()) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (!wait(bP + 16 * x + 8 * h, j & 1)) break;
-                    fence_after_sync();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 4 * h; k < 4 * h + 4; ++k)
-                            mma_ts(tO, tP + k * 8, dv + at + (k * 2048 >> 4), id_o, j > 0 || k > 0);
-                        if (h == 1) {
-                            mma_commit(bPV + 8 * x);
-                            if (j + 1 >= n) mma_commit(bEmpty + 8 * s);
+                            for (int d = 0; d < DP / 16; ++d) {
+                                const uint32_t at = (d / 4 * C::HALF_BYTES + d % 4 * 32) >> 4;
+                                mma_ss(tm + C::S0, dq + (x * C::TILE_BYTES >> 4) + at, k + at, id, d > 0);
+                            }
+                            mma_commit(bS + 8 * x);
                         }
+                        __syncwarp();
                     }
+                    if (ok && elect_one()) mma_commit(bEmpty + 8 * s);
                     __syncwarp();
                 }
-                if (ok && j + 1 < n && (!C::P_OVER_S || wait(bPV + 8 * x, j & 1))) score(dk + at, s);
+            } else {
+                constexpr uint32_t id = idesc_of(BF16, 1, DP);
+                const uint32_t dv = desc_lo(base + 2 * C::TILE_BYTES, C::HALF_BYTES);
+                if (all > 0) {  // pair 0 has no V
+                    if (elect_one()) mbar_arrive(bEmpty);
+                    __syncwarp();
+                }
+                const int r_lo = (int)max(min(lo - k0, (int64_t)kTile), (int64_t)0);  // rows of step 0 below the keys
+                for (int j = 0; j < all && ok; ++j) {
+                    const int s = (j + 1) % kStages;  // V of step j is in pair j + 1
+                    if (!wait(bFull + 8 * s, (j + 1) / kStages & 1)) break;
+                    // the rows of V outside the block's keys become 0
+                    const int r_hi = (int)min(k1 - k0 - (int64_t)j * kTile, (int64_t)kTile);
+                    if ((j == 0 && r_lo > 0) || r_hi < kTile) {
+                        uint8_t *v = sKV + 2 * s * C::TILE_BYTES;
+                        for (int e = lane; e < kTile * HALVES * 8; e += 32) {
+                            const int row = (e >> 3) % kTile, h = e / (kTile * 8);
+                            if ((j == 0 && row < r_lo) || row >= r_hi)
+                                *reinterpret_cast<uint4 *>(v + h * C::HALF_BYTES + row * 128 + (e & 7) * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    const uint32_t v = dv + 2 * s * (C::TILE_BYTES >> 4);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (j >= (x ? n1 : n0)) continue;
+                        // O += P V, the first 64 keys as soon as their weights are there
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (!wait(bP + 16 * x + 8 * h, j & 1)) break;
+                            fence_after_sync();
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 4 * h; k < 4 * h + 4; ++k)
+                                    mma_ts(tm + C::O0 + x * DP, tm + C::P0 + x * (kTile / 2) + k * 8,
+                                           v + (k * 2048 >> 4), id, j > 0 || k > 0);
+                                if (h == 1) mma_commit(bPV + 8 * x);
+                            }
+                            __syncwarp();
+                        }
+                        if (!ok) break;
+                    }
+                    if (ok && elect_one()) mma_commit(bEmpty + 8 * s);
+                    __syncwarp();
+                }
             }
             // every MMA issued has completed before tensor memory is freed
-            if (elect_one()) mma_commit(bDrain + 8 * x);
+            const uint32_t drain = bDrain + (warp == kValueWarp ? 8 : 0);
+            if (elect_one()) mma_commit(drain);
             __syncwarp();
-            mbar_wait(bDrain + 8 * x, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
+            mbar_wait(drain, 0, a.err, kErrPagedWait, TC_DRAIN_NS);
         }
         asm volatile("bar.sync 0;" ::: "memory");
-        if (warp == kMmaWarp) {
+        if (warp == kScoreWarp) {
             fence_after_sync();
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
         }
@@ -391,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
         const int x = warp >> 2, row = tid & (kTile - 1);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
-        const uint32_t tS = tmem + C::S0 + x * kTile + lanes, tO = tmem + C::O0 + x * DP + lanes,
-                       tP = tmem + C::P0 + x * C::P_STEP + lanes;
+        const uint32_t tS = tmem + C::S0 + lanes, tO = tmem + C::O0 + x * DP + lanes,
+                       tP = tmem + C::P0 + x * (kTile / 2) + lanes;
         const int i = row / group;
         const bool live = i < n_tok[x] && row < tile_tok * group;
         const int64_t tq = t.tok0 + tok[x] + i;
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool flip = a.scale < 0.f;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        const int n = x ? n_step[1] : n_step[0], n_other = x ? n_step[0] : n_step[1];
+        const int n = x ? n_step[1] : n_step[0];
         // whether a page of the block's keys is missing, looked up while the
         // first copies are under way
         bool gone = false;
@@ -420,9 +424,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < n && ok; ++j) {
             const int c0 = see_lo - j * kTile, c1 = see_hi - j * kTile;  // the columns seen, [c0, c1)
             ok = mbar_wait_tight(bS + 8 * x, j & 1, a.err, kErrPagedWait);
-            // the product of the step before is complete too (P_OVER_S: the
-            // issuer waited for it); its barrier's phases are taken in turn
-            if (!C::P_OVER_S && j > 0 && ok) ok = mbar_wait_tight(bPV + 8 * x, (j - 1) & 1, a.err, kErrPagedWait);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after_sync();
@@ -430,6 +431,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < kTile; c += 32) tmem_get32(tS + c, s + c);
             tmem_get_wait();
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bFree);
             if (flip) {
 #pragma unroll
                 for (int c = 0; c < kTile; ++c) s[c] = -s[c];
@@ -454,20 +458,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            // The softmax of the two tiles takes turns, A 0, B 0, A 1, ...: in
-            // step with one another, both tiles would wait for the tensor
-            // cores at the same time, and then both for the exponentials.
-            if (ok && (x ? j < n_other : j > 0 && j - 1 < n_other))
-                ok = mbar_wait_tight(bTurn + 8 * (x ^ 1), (x ? j : j - 1) & 1, a.err, kErrPagedWait);
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
             for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
             const float m_new = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
+            // P and O of the step before have been read and written
+            if (j > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait_tight(bPV + 8 * x, (j - 1) & 1, a.err, kErrPagedWait));
+                if (!ok) break;
+                fence_after_sync();
+            }
             if (j == 0) {
                 m = m_new;
             } else if (__any_sync(0xffffffffu, (m_new - m) * sc > kGrow)) {
-                // O of the steps before is complete: the commit behind this
-                // step's S covers their products too
                 const float f = m_new == m ? 1.f : pow2((m - m_new) * sc);
                 m = m_new;
                 l *= f;
@@ -496,10 +499,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     u[e] = pack2(p.x, p.y, T());
                 }
                 tmem_put32(tP + c / 2, u);
-                if (c > 0) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bTurn + 8 * x);
-                }
                 tmem_put_wait();
                 fence_before_sync();
                 __syncwarp();
