@@ -455,8 +455,9 @@ typedef struct kk_paged_cache {
  *   positions  [n_tokens] position of each new token in its request (may be
  *              NULL)
  *   status     [3] the free range that is left (two values, as free_range of
- *              the next call) and how many pages were missing; must not
- *              overlap free_range
+ *              the next call) and how many pages were missing
+ * Outputs do not overlap inputs (status and free_range, seq_len and ctx_len
+ * are checked).
  * n_tokens is at least the number of new tokens: rows of slots and positions
  * past it are set to -1, tokens past n_tokens get neither slots nor pages in
  * the table (though status counts their pages). */
@@ -490,11 +491,15 @@ int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_t
  * product with v.
  *   max_new, max_len: the largest number of new tokens and of cached tokens
  * of a request. They choose how the work is divided; results are right for
- * any values. Rows of out past the last new token are left as they were.
- * Few rows over a long cache are worked on in pieces through a workspace of
- * the context: such a call is ordered after the context's previous call, like
- * the other entry points. While the stream is being captured the keys are
- * not divided. */
+ * any values. Rows of out past the last new token are left as they were. out
+ * does not overlap q or the cache. Positions past 2^31 - 1024 are not
+ * attended to.
+ * Where there are too few rows for the GPU, the keys are divided and the
+ * pieces joined through a workspace of the context: such a call is ordered
+ * after the context's previous call, like the other entry points. While the
+ * stream is being captured the keys are not divided. Every wait inside is
+ * bounded; one that ran out is reported (KK_ERROR_INFERENCE) by the next call
+ * of the context that synchronises. */
 int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t n_seqs, const int32_t *seq_len,
                               const int32_t *cu_new, int64_t n_tokens, int32_t max_new, int32_t max_len,
                               const int32_t *table, int32_t max_pages, const void *q, int64_t q_stride,
@@ -507,7 +512,8 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
  * and 2 i + 1 in the high one; scales: IEEE half [n_out][n_in / group]; group
  * 32, 64 or 128, n_in a multiple of it; x and out of `dtype` (F32, F16 or
  * BF16), rows x_stride and out_stride values apart, w and the rows of x
- * 16-byte aligned; bias F32 or NULL. Products are exact and sums 32-bit. */
+ * 16-byte aligned; bias F32 or NULL. Products are exact and sums 32-bit. A
+ * bounded wait that ran out is reported as above. */
 int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in, int32_t group, const uint8_t *w,
                         const uint16_t *scales, int32_t dtype, const void *x, int64_t x_stride, const float *bias,
                         void *out, int64_t out_stride, void *stream);

@@ -22,7 +22,9 @@ namespace kk {
 // passes), then writes its share of the tokens, 32 of a warp, which find their
 // requests by searching the scanned offsets in shared memory. The token at
 // the start of a new page writes the table entry, so no block reads what
-// another writes.
+// another writes. Measured on B200: 64 requests of one token 10 us a call, the
+// host's; 2048 requests with 1.05 M tokens 14.5 us (13 MB, 2 us of traffic:
+// the scan in every block and the searches bound it).
 // ---------------------------------------------------------------------------
 constexpr int kPtThreads = 1024;
 constexpr int kPtPer = 4;
@@ -176,7 +178,8 @@ cudaError_t page_tables(const PageTablesArgs &a, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // Append: row t of k and v (n_kv_heads x head_dim values, rows apart by their
 // strides) to the cache row of slots[t]; a slot outside the cache is skipped.
-// A copy: bytes bound it. A thread moves 8 values of K and the same 8 of V,
+// A copy: bytes bound it (16381 tokens of 12 heads of 64, F32 to F16, 151 MB
+// in 27.4 us, 5.5 TB/s). A thread moves 8 values of K and the same 8 of V,
 // 16-byte stores into the cache and 16- or 32-byte loads from the source.
 // ---------------------------------------------------------------------------
 template <typename T>

@@ -40,6 +40,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
         : "memory");
 }
 
+// Keys that a request's table can hold; positions and steps past them fit 32
+// bits.
+__device__ __forceinline__ int64_t paged_capacity(const PagedAttnArgs &a) {
+    return min((int64_t)a.max_pages * a.cache.page_size, (int64_t)INT32_MAX - 1023);
+}
+
 // The tile `w` of a launch, `unit` rows (query, head of the group) each.
 // Request r's tiles begin at floor(cu[r] * group / unit) + r: consecutive
 // requests are at least as far apart as request r has tiles, so the request

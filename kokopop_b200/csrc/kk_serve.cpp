@@ -19,6 +19,11 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 bool dtype16(int dtype) { return dtype == KK_DTYPE_F16 || dtype == KK_DTYPE_BF16; }
 bool dtype_any(int dtype) { return dtype == KK_DTYPE_F32 || dtype16(dtype); }
 
+// whether [a, a + n) and [b, b + m) have nothing in common
+bool apart(const int32_t *a, int64_t n, const int32_t *b, int64_t m) {
+    return (uintptr_t)(a + n) <= (uintptr_t)b || (uintptr_t)(b + m) <= (uintptr_t)a;
+}
+
 constexpr int64_t kMaxTokens = INT32_MAX / 2;  // rows of one call
 
 PagedCacheView cache_view(const kk_paged_cache *c) {
@@ -95,8 +100,10 @@ int kk_page_tables_device(kk_ctx *ctx, int32_t n_seqs, int32_t page_size, int32_
         need(n_free >= 0 && (free_pages || n_free == 0), "null free_pages or negative n_free");
         need(n_tokens >= 0 && n_tokens <= kMaxTokens, "n_tokens out of range");
         need(slots || n_tokens == 0, "null slots");
-        need((uintptr_t)(free_range + 2) <= (uintptr_t)status || (uintptr_t)(status + 3) <= (uintptr_t)free_range,
-             "status overlaps free_range");
+        need(apart(status, 3, free_range, 2), "status overlaps free_range");
+        need(apart(seq_len, n_seqs, ctx_len, n_seqs) && apart(seq_len, n_seqs, new_len, n_seqs) &&
+                 apart(cu_new, n_seqs + 1ll, ctx_len, n_seqs) && apart(cu_new, n_seqs + 1ll, new_len, n_seqs),
+             "seq_len or cu_new overlaps ctx_len or new_len");
         use_device(ctx);
         PageTablesArgs a;
         a.n_seqs = n_seqs;

@@ -19,7 +19,7 @@ def _cache(**kw):
 
 def _tables(**kw):
     a = dict(ctx=P, n_seqs=2, page_size=16, max_pages=4, ctx_len=P, new_len=P, free_pages=P, n_free=8, free_range=P,
-             table=P, seq_len=P, cu_new=P, n_tokens=2, slots=P, positions=P, status=P + 64, stream=0)
+             table=P, seq_len=P + 32, cu_new=P + 48, n_tokens=2, slots=P, positions=P, status=P + 64, stream=0)
     a.update(kw)
     return kb.load_library().kk_page_tables_device(*a.values())
 
@@ -54,7 +54,8 @@ BAD_CACHE = [dict(k_ptr=0), dict(v_ptr=0), dict(k_ptr=P + 8), dict(dtype=kb.DTYP
     (_tables, b) for b in (dict(ctx=None), dict(ctx_len=None), dict(new_len=None), dict(free_pages=None),
                            dict(free_range=None), dict(table=None), dict(seq_len=None), dict(cu_new=None),
                            dict(slots=None), dict(status=None), dict(n_seqs=0), dict(page_size=0), dict(max_pages=0),
-                           dict(n_free=-1), dict(n_tokens=-1), dict(status=P + 4), dict(free_range=P + 72))
+                           dict(n_free=-1), dict(n_tokens=-1), dict(status=P + 4), dict(free_range=P + 72),
+                           dict(seq_len=P + 4), dict(cu_new=P), dict(new_len=P + 36), dict(ctx_len=P + 56))
 ] + [
     (_append, b) for b in (dict(ctx=None), dict(cache=None), dict(slots=None), dict(k=None), dict(v=None),
                            dict(n_tokens=-1), dict(dtype=7), dict(k=P + 4), dict(k_stride=120), dict(v_stride=130),
