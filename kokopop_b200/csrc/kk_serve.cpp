@@ -204,12 +204,16 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         a.err = (int *)ctx->d_err.p;
         // pieces of the key axis, from the largest lengths that the caller names
         const int64_t rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
-        const int64_t blocks = std::min(plan.tiles, n_seqs * ((rows + plan.unit - 1) / plan.unit)) * a.cache.n_kv_heads;
+        // (all rows are in some tile, whatever max_new says)
+        const int64_t least = (n_tokens * group + plan.unit - 1) / plan.unit;
+        const int64_t blocks =
+            std::max(least, std::min(plan.tiles, n_seqs * ((rows + plan.unit - 1) / plan.unit))) * a.cache.n_kv_heads;
         int64_t keys = std::max(max_len, 1);
         if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + plan.unit / group + 16);
         a.splits = capturing(st) ? 1 : plan.chunk ? chunk_pieces(blocks, keys) : row_pieces(blocks, keys);
         const int64_t step = plan.chunk ? 128 : 64;
-        a.split_keys = (int)(((keys + a.splits - 1) / a.splits + step - 1) / step * step);
+        a.split_keys = (int)std::min<int64_t>(((keys + a.splits - 1) / a.splits + step - 1) / step * step,
+                                              INT32_MAX / 128 * 128);
         if (a.splits == 1) {
             check_cuda(paged_attn(plan, a, st), "paged attention launch");
             ++ctx->n_launches;
@@ -226,7 +230,9 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
             const size_t count_bytes = (size_t)plan.tiles * a.cache.n_kv_heads * sizeof(unsigned);
             if (count.bytes < count_bytes) {
                 count.ensure(count_bytes);
-                check_cuda(cudaMemsetAsync(count.p, 0, count.bytes, st), "clear the piece counters");
+                const cudaError_t e = cudaMemsetAsync(count.p, 0, count.bytes, st);
+                if (e != cudaSuccess) count.release();  // not to be taken for cleared
+                check_cuda(e, "clear the piece counters");
             }
             a.count = (unsigned *)count.p;
         }
