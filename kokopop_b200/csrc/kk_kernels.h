@@ -418,7 +418,9 @@ struct PagedAttnPlan {
     int unit;
     int64_t tiles;
 };
-PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new);
+// keys: at most that many are seen by a query.
+PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new,
+                              int64_t keys);
 cudaError_t paged_attn(const PagedAttnPlan &p, const PagedAttnArgs &a, cudaStream_t st);
 // kk_paged_chunk.cu
 bool paged_chunk_serves(const PagedCacheView &c, int n_heads);

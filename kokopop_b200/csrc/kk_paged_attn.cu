@@ -517,11 +517,21 @@ static cudaError_t launch_row_of(const PagedAttnPlan &p, const PagedAttnArgs &a,
     return tma ? launch_row<T, DP, 2, true>(a, p.tiles, st) : launch_row<T, DP, 2, false>(a, p.tiles, st);
 }
 
-PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new) {
+// Chunks of queries take the chunk kernel, whose blocks read the keys once for
+// 256 rows but start and end slowly (about 5 us). Up to 48 rows over few keys
+// in many requests, the row kernel's smaller blocks are done sooner although
+// they read the keys up to three times: 105 requests of 18-41 new tokens, 16
+// heads, 41-410 keys 131 us against 157; 80 of 3-4 tokens, 8 heads on each of
+// 4, a window of 487 keys 39 against 52. With less than two rounds of chunk
+// blocks there is nothing to win: 32 requests of 5 tokens, 4 heads on each of 8,
+// 500-2000 keys 76 against 75; 45 of 8-13 tokens, 8 heads on one 38 against 24.
+PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new,
+                              int64_t keys) {
     const int group = n_heads / c.n_kv_heads;
     const int64_t rows = (n_tokens < max_new ? n_tokens : max_new) * (int64_t)group;
+    const bool short_rows = rows <= 48 && keys <= 1024 && (int64_t)n_seqs * c.n_kv_heads >= 2 * 148;
     PagedAttnPlan p;
-    p.chunk = rows > kFewRows && paged_chunk_serves(c, n_heads);
+    p.chunk = rows > kFewRows && !short_rows && paged_chunk_serves(c, n_heads);
     p.unit = p.chunk ? paged_chunk_unit(group) : rows > 8 ? 16 : 8;
     p.tiles = n_tokens * group / p.unit + n_seqs;
     return p;

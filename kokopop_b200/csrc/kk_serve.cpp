@@ -179,7 +179,9 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         need(q_stride >= row && out_stride >= row && q_stride % 8 == 0 && out_stride % 8 == 0,
              "q and out strides must hold a row and be multiples of 8 values");
         const int group = n_heads / a.cache.n_kv_heads;
-        const PagedAttnPlan plan = paged_attn_plan(a.cache, n_heads, n_tokens, n_seqs, max_new);
+        int64_t keys = std::max(max_len, 1);  // that a query sees, from the lengths that the caller names
+        if (window > 0) keys = std::min<int64_t>(keys, window);
+        const PagedAttnPlan plan = paged_attn_plan(a.cache, n_heads, n_tokens, n_seqs, max_new, keys);
         need(plan.tiles <= INT32_MAX && n_tokens * group <= INT32_MAX,
              "n_tokens x query heads per key head out of range");
         use_device(ctx);
@@ -202,14 +204,13 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         a.count = nullptr;
         a.part_n = nullptr;
         a.err = (int *)ctx->d_err.p;
-        // pieces of the key axis, from the largest lengths that the caller names
+        // pieces of the key axis
         const int64_t rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
         // (all rows are in some tile, whatever max_new says)
         const int64_t least = (n_tokens * group + plan.unit - 1) / plan.unit;
         const int64_t blocks =
             std::max(least, std::min(plan.tiles, n_seqs * ((rows + plan.unit - 1) / plan.unit))) * a.cache.n_kv_heads;
-        int64_t keys = std::max(max_len, 1);
-        if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + plan.unit / group + 16);
+        if (window > 0) keys = std::min<int64_t>(std::max(max_len, 1), (int64_t)window + plan.unit / group + 16);
         a.splits = capturing(st) ? 1 : plan.chunk ? chunk_pieces(blocks, keys) : row_pieces(blocks, keys);
         const int64_t step = plan.chunk ? 128 : 64;
         a.split_keys = (int)std::min<int64_t>(((keys + a.splits - 1) / a.splits + step - 1) / step * step,

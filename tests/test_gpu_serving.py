@@ -296,6 +296,15 @@ def test_attention_over_a_long_cache_in_pieces(ctx, window, new):
     _attend_check(ctx, [5003, 2100], [new, 1], 8, 2, 128, 32, window, "token", "bf16")
 
 
+@pytest.mark.parametrize("window", [0, 30])
+def test_attention_of_many_short_requests(ctx, window):
+    """Enough requests and few enough rows and keys for the row kernel."""
+    rng = np.random.default_rng(7)
+    new = rng.integers(1, 13, 80).tolist()
+    lens = [int(n + rng.integers(0, 90)) for n in new]
+    _attend_check(ctx, lens, new, 16, 4, 64, 16, window, "token", "bf16")
+
+
 def test_attention_hints_do_not_change_what_is_computed(ctx):
     """max_new and max_len only choose the division of the work: too small
     or too large, the result is within the same tolerances."""
