@@ -30,7 +30,7 @@
 //
 // Measured on B200, 32 heads of 128 on 8, one token each: 7 requests of
 // 30011-65000 keys 216 us, 6.8 TB/s of cache read (the copy rate is 6.55); 64
-// requests of 17-4099 keys 98 us, 5.2 TB/s, where blocks start and end unevenly.
+// requests of 17-4099 keys 97 us, 5.3 TB/s, where blocks start and end unevenly.
 #include "kk_paged_attn.cuh"
 #include "kk_ptx.cuh"
 
@@ -148,8 +148,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t cap = paged_capacity(a);
     const int64_t lo = a.window > 0 ? max((int64_t)pos_first - a.window + 1, (int64_t)0) : 0;
     const int64_t kbeg = lo / kKeys * kKeys, kend = max(min((int64_t)pos_last + 1, cap), kbeg);
-    int64_t piece = (kend - kbeg + a.splits - 1) / a.splits;
-    piece = max((piece + 63) / 64 * 64, (int64_t)a.split_keys);
+    // pieces: at most `splits`, of split_keys keys or more, then of one size
+    const int64_t most = max((kend - kbeg + a.splits - 1) / a.splits, (int64_t)a.split_keys);
+    const int64_t parts = max((kend - kbeg + most - 1) / most, (int64_t)1);
+    const int64_t piece = max(((kend - kbeg + parts - 1) / parts + 63) / 64 * 64, (int64_t)64);
     const int n_pieces = (int)max((kend - kbeg + piece - 1) / piece, (int64_t)1);
     const int sp = blockIdx.z;
     if (sp >= n_pieces) return;

@@ -193,8 +193,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int64_t lo = a.window > 0 ? max((int64_t)t.base + tok_first - a.window + 1, (int64_t)0) : 0;
     const int64_t kbeg = lo / kTile * kTile, kend = max(max(hi[0], hi[1]), kbeg);
-    int64_t piece = (kend - kbeg + a.splits - 1) / a.splits;
-    piece = max((piece + kTile - 1) / kTile * kTile, (int64_t)a.split_keys);
+    // pieces: at most `splits`, of split_keys keys or more, then of one size
+    const int64_t most = max((kend - kbeg + a.splits - 1) / a.splits, (int64_t)a.split_keys);
+    const int64_t parts = max((kend - kbeg + most - 1) / most, (int64_t)1);
+    const int64_t piece = max(((kend - kbeg + parts - 1) / parts + kTile - 1) / kTile * kTile, (int64_t)kTile);
     const int n_pieces = (int)max((kend - kbeg + piece - 1) / piece, (int64_t)1);
     const int sp = blockIdx.z;
     if (sp >= n_pieces) return;
