@@ -146,8 +146,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int rows_here = min(C::ROWS, t.rows - t.row0);
     const int pos_first = t.base + t.row0 / group, pos_last = t.base + (t.row0 + rows_here - 1) / group;
     const int64_t cap = paged_capacity(a);
-    const int64_t lo = a.window > 0 ? max((int64_t)pos_first - a.window + 1, (int64_t)0) : 0;
-    const int64_t kbeg = lo / kKeys * kKeys, kend = max(min((int64_t)pos_last + 1, cap), kbeg);
+    // (a window wholly past the table leaves the block no key: k0 = k1, and no
+    // step of the ring lies past 2^31)
+    const int64_t lo = a.window > 0 ? min(max((int64_t)pos_first - a.window + 1, (int64_t)0), cap) : 0;
+    const int64_t kbeg = lo / kKeys * kKeys, kend = lo < cap ? max(min((int64_t)pos_last + 1, cap), kbeg) : kbeg;
     // pieces: at most `splits`, of split_keys keys or more, then of one size
     const int64_t most = max((kend - kbeg + a.splits - 1) / a.splits, (int64_t)a.split_keys);
     const int64_t parts = max((kend - kbeg + most - 1) / most, (int64_t)1);

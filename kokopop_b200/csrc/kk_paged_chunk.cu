@@ -191,8 +191,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         n_tok[x] = max(min(t.n - tok[x], tile_tok), 0);
         hi[x] = n_tok[x] > 0 ? max(min((int64_t)t.base + tok[x] + n_tok[x], cap), (int64_t)0) : 0;
     }
-    const int64_t lo = a.window > 0 ? max((int64_t)t.base + tok_first - a.window + 1, (int64_t)0) : 0;
-    const int64_t kbeg = lo / kTile * kTile, kend = max(max(hi[0], hi[1]), kbeg);
+    // (a window wholly past the table leaves the block no key: k0 = k1)
+    const int64_t lo = a.window > 0 ? min(max((int64_t)t.base + tok_first - a.window + 1, (int64_t)0), cap) : 0;
+    const int64_t kbeg = lo / kTile * kTile, kend = lo < cap ? max(max(hi[0], hi[1]), kbeg) : kbeg;
     // pieces: at most `splits`, of split_keys keys or more, then of one size
     const int64_t most = max((kend - kbeg + a.splits - 1) / a.splits, (int64_t)a.split_keys);
     const int64_t parts = max((kend - kbeg + most - 1) / most, (int64_t)1);
@@ -419,9 +420,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         const int n = x ? n_step[1] : n_step[0];
         // whether a page of the block's keys is missing, looked up while the
-        // first copies are under way
+        // first copies are under way; without a step there is no page to look up
         bool gone = false;
-        for (int64_t key = k0 / page_size * page_size + (int64_t)tid * page_size; key < k1;
+        for (int64_t key = k0 / page_size * page_size + (int64_t)tid * page_size; steps > 0 && key < k1;
              key += (int64_t)2 * kTile * page_size) {
             const int page = table[(int)key / page_size];
             gone |= page < 0 || page >= a.cache.n_pages;
