@@ -431,7 +431,8 @@ int kk_vocos_forward_device(kk_ctx *ctx, const char *prefix, const kk_vocos_para
  * same strides), so [page][token][head][d] and [page][head][token][d] are
  * both served. k and v are 16-byte aligned, the strides multiples of 8
  * values, head_dim a multiple of 8 up to KK_PAGED_MAX_HEAD_DIM. A slot is
- * page * page_size + token. */
+ * page * page_size + token. A call takes at most 2^30 - 1 requests and new
+ * tokens. */
 #define KK_PAGED_MAX_HEAD_DIM 128
 typedef struct kk_paged_cache {
     void *k, *v;
@@ -512,7 +513,8 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
  * and 2 i + 1 in the high one; scales: IEEE half [n_out][n_in / group]; group
  * 32, 64 or 128, n_in a multiple of it; x and out of `dtype` (F32, F16 or
  * BF16), rows x_stride and out_stride values apart, w and the rows of x
- * 16-byte aligned; bias F32 or NULL. Products are exact and sums 32-bit. A
+ * 16-byte aligned; bias F32 or NULL; at most 524280 rows, n_out and n_in at
+ * most 2^31 - 65536. Products are exact and sums 32-bit. A
  * bounded wait that ran out is reported as above. */
 int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in, int32_t group, const uint8_t *w,
                         const uint16_t *scales, int32_t dtype, const void *x, int64_t x_stride, const float *bias,

@@ -24,7 +24,10 @@ bool apart(const int32_t *a, int64_t n, const int32_t *b, int64_t m) {
     return (uintptr_t)(a + n) <= (uintptr_t)b || (uintptr_t)(b + m) <= (uintptr_t)a;
 }
 
-constexpr int64_t kMaxTokens = INT32_MAX / 2;  // rows of one call
+constexpr int64_t kMaxTokens = INT32_MAX / 2;  // rows, or requests, of one call
+// outputs and inputs of a product: the kernel's 32-bit indices reach a chunk
+// of k and a block of outputs further
+constexpr int32_t kMaxSide = INT32_MAX - 65535;
 
 PagedCacheView cache_view(const kk_paged_cache *c) {
     need(c && c->k && c->v, "null cache");
@@ -97,6 +100,7 @@ int kk_page_tables_device(kk_ctx *ctx, int32_t n_seqs, int32_t page_size, int32_
     return guarded([&] {
         need(ctx && ctx_len && new_len && free_range && table && seq_len && cu_new && status, "null argument");
         need(n_seqs >= 1 && page_size >= 1 && max_pages >= 1, "n_seqs, page_size or max_pages below 1");
+        need(n_seqs <= kMaxTokens, "n_seqs out of range");
         need(n_free >= 0 && (free_pages || n_free == 0), "null free_pages or negative n_free");
         need(n_tokens >= 0 && n_tokens <= kMaxTokens, "n_tokens out of range");
         need(slots || n_tokens == 0, "null slots");
@@ -168,6 +172,7 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         need(seq_len && cu_new && table, "null argument");
         need(n_seqs >= 1 && max_pages >= 1 && max_new >= 0 && max_len >= 0,
              "n_seqs or max_pages below 1, or a negative max_new or max_len");
+        need(n_seqs <= kMaxTokens, "n_seqs out of range");
         need(n_tokens >= 0 && n_tokens <= kMaxTokens, "n_tokens out of range");
         need(n_heads >= 1 && n_heads % a.cache.n_kv_heads == 0, "n_heads is not a multiple of the cache's n_kv_heads");
         need(scale == scale, "scale is not a number");
@@ -248,7 +253,9 @@ int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in
                         void *out, int64_t out_stride, void *stream) {
     return guarded([&] {
         need(ctx && w && scales, "null argument");
-        need(n_rows >= 0 && n_rows <= 8 * 65535 && n_out >= 1 && n_in >= 1, "n_rows, n_out or n_in out of range");
+        need(n_rows >= 0 && n_rows <= 8 * 65535 && n_out >= 1 && n_out <= kMaxSide && n_in >= 1 &&
+                 n_in <= kMaxSide,
+             "n_rows, n_out or n_in out of range");
         need(group == 32 || group == 64 || group == 128, "group is not 32, 64 or 128");
         need(n_in % group == 0, "n_in is not a multiple of the group");
         need(dtype_any(dtype), "dtype is not F32, F16 or BF16");

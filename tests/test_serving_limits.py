@@ -1,0 +1,23 @@
+"""Arguments of the serving operators that no kernel could take safely are
+refused before a GPU is touched."""
+import pytest
+
+import kokopop_b200 as kb
+from test_serving_abi import P, _append, _attend, _q4, _tables
+
+TOP = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("call,bad", [
+    (_tables, dict(n_seqs=2 ** 30, n_free=0, seq_len=P + 2 ** 34, cu_new=P + 2 ** 35, status=P + 2 ** 36)),
+    (_attend, dict(n_seqs=2 ** 30)),
+    (_attend, dict(n_seqs=TOP)),
+    # a chunk of k, or a block of outputs, past the last one would not fit 32 bits
+    (_q4, dict(n_in=TOP // 128 * 128, x_stride=2 ** 31)),
+    (_q4, dict(n_in=2 ** 31 - 65408, x_stride=2 ** 31)),
+    (_q4, dict(n_out=TOP, out_stride=2 ** 31)),
+    (_q4, dict(n_out=2 ** 31 - 65535, out_stride=2 ** 31)),
+])
+def test_sizes_whose_indices_pass_32_bits_are_refused(call, bad):
+    assert call(**bad) == kb.KK_ERROR_INVALID_ARGUMENT
+    assert "out of range" in kb.load_library().kk_last_error().decode()
