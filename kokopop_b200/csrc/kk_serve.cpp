@@ -16,6 +16,8 @@ void need(bool ok, const char *m) {
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+bool aligned4(const int32_t *p) { return ((uintptr_t)p & 3) == 0; }
+bool aligned8(const int64_t *p) { return ((uintptr_t)p & 7) == 0; }
 bool dtype16(int dtype) { return dtype == KK_DTYPE_F16 || dtype == KK_DTYPE_BF16; }
 bool dtype_any(int dtype) { return dtype == KK_DTYPE_F32 || dtype16(dtype); }
 
@@ -104,6 +106,10 @@ int kk_page_tables_device(kk_ctx *ctx, int32_t n_seqs, int32_t page_size, int32_
         need(n_free >= 0 && (free_pages || n_free == 0), "null free_pages or negative n_free");
         need(n_tokens >= 0 && n_tokens <= kMaxTokens, "n_tokens out of range");
         need(slots || n_tokens == 0, "null slots");
+        need(aligned4(ctx_len) && aligned4(new_len) && aligned4(free_pages) && aligned4(free_range) &&
+                 aligned4(table) && aligned4(seq_len) && aligned4(cu_new) && aligned4(positions) && aligned4(status) &&
+                 aligned8(slots),
+             "an argument is not aligned to its type");
         need(apart(status, 3, free_range, 2), "status overlaps free_range");
         need(apart(seq_len, n_seqs, ctx_len, n_seqs) && apart(seq_len, n_seqs, new_len, n_seqs) &&
                  apart(cu_new, n_seqs + 1ll, ctx_len, n_seqs) && apart(cu_new, n_seqs + 1ll, new_len, n_seqs),
@@ -142,6 +148,7 @@ int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_t
         need(dtype_any(dtype), "dtype is not F32, F16 or BF16");
         if (n_tokens == 0) return KK_OK;
         need(slots && k && v, "null argument");
+        need(aligned8(slots), "slots is not aligned to its type");
         const int64_t row = (int64_t)a.cache.n_kv_heads * a.cache.head_dim, step = dtype == KK_DTYPE_F32 ? 4 : 8;
         need(aligned16(k) && aligned16(v), "k and v must be 16-byte aligned");
         need(k_stride >= row && v_stride >= row && k_stride % step == 0 && v_stride % step == 0,
@@ -170,6 +177,8 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         PagedAttnArgs a;
         a.cache = cache_view(cache);
         need(seq_len && cu_new && table, "null argument");
+        need(aligned4(seq_len) && aligned4(cu_new) && aligned4(table),
+             "seq_len, cu_new or table is not aligned to its type");
         need(n_seqs >= 1 && max_pages >= 1 && max_new >= 0 && max_len >= 0,
              "n_seqs or max_pages below 1, or a negative max_new or max_len");
         need(n_seqs <= kMaxTokens, "n_seqs out of range");

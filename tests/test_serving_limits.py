@@ -21,3 +21,13 @@ TOP = 2 ** 31 - 1
 def test_sizes_whose_indices_pass_32_bits_are_refused(call, bad):
     assert call(**bad) == kb.KK_ERROR_INVALID_ARGUMENT
     assert "out of range" in kb.load_library().kk_last_error().decode()
+
+
+@pytest.mark.parametrize("call,bad", [
+    (_tables, {name: P + 2 ** 20 + 2}) for name in ("ctx_len", "new_len", "free_pages", "free_range", "table", "seq_len",
+                                                    "cu_new", "positions", "status")
+] + [(_attend, {name: P + 2}) for name in ("seq_len", "cu_new", "table")] + [(c, dict(slots=P + 4))
+                                                                            for c in (_tables, _append)])
+def test_arrays_that_are_not_aligned_to_their_type_are_refused(call, bad):
+    assert call(**bad) == kb.KK_ERROR_INVALID_ARGUMENT
+    assert "aligned" in kb.load_library().kk_last_error().decode()
