@@ -489,7 +489,8 @@ int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_t
  * anything, NaN included; a NaN or infinite value of a token that one query
  * sees can reach earlier queries of the same chunk. Scores, sums and maxima
  * are 32-bit; the softmax weights are rounded to the cache's type for the
- * product with v.
+ * product with v (half: relative to 2^-7 of the largest, so that they are
+ * normal numbers from 2^-21 of it on).
  *   max_new, max_len: the largest number of new tokens and of cached tokens
  * of a request. They choose how the work is divided; results are right for
  * any values. Rows of out past the last new token are left as they were. out

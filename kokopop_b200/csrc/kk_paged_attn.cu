@@ -10,7 +10,9 @@
 // Scores, maxima, sums and the output are 32-bit; the weights e^(s - m) are
 // rounded once to the cache's 16-bit type, which is what the tensor cores
 // multiply (their relative error, 2^-8 or 2^-11 at most, is that of the
-// rounded output), while the sum in the denominator takes them unrounded.
+// rounded output; in half, weights below 2^-21 of the largest are rounded to
+// multiples of 2^-31 of it), while the sum in the denominator takes them
+// unrounded.
 //
 // k_paged_attn_row: for one or a few queries per key head, bytes bound it:
 // every key and value of the request is read once for the `group` heads that
@@ -367,7 +369,8 @@ __global__ void __launch_bounds__(kWarps * 32)
         uint32_t p[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const float r0 = mx[b][0] == -INFINITY ? 0.f : mx[b][0], r1 = mx[b][1] == -INFINITY ? 0.f : mx[b][1];
+            const float r0 = (mx[b][0] == -INFINITY ? 0.f : mx[b][0]) - kLift<T>,
+                        r1 = (mx[b][1] == -INFINITY ? 0.f : mx[b][1]) - kLift<T>;
             const float x0 = pow2(sc[b][0] - r0), x1 = pow2(sc[b][1] - r1);
             const float y0 = pow2(sc[b][2] - r0), y1 = pow2(sc[b][3] - r1);
             sum[b][0] += x0 + y0;

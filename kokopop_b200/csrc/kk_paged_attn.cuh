@@ -20,7 +20,18 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// 2^x, results below 2^-126 as 0 (weights are at most 2^8 and rounded to 16
+// The weights of the product with V are 2^(s - m + kLift): half has 2^-14 as
+// its smallest normal number, and weights that are small fractions of the
+// largest one count where the keys are many. m is at most 8 behind the
+// maximum, so half's reach 2^15 (its largest is 2^16 - 32), and they are
+// normal from 2^-21 of the largest on. The factor is in the sums too and
+// leaves with the division; bfloat16 has the range of 32 bits and needs none.
+template <typename T>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<__half> = 7.f;
+
+// 2^x, results below 2^-126 as 0 (weights are at most 2^15 and rounded to 16
 // bits, or relative to a largest one)
 __device__ __forceinline__ float pow2(float x) {
     float r;

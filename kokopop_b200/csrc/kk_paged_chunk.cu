@@ -15,9 +15,9 @@
 // another product; P has columns of its own. (With an S for each tile and P
 // over it, the next S waited for the product that reads P: 485 us where this
 // takes 444.) m follows the running maximum lazily: O is rescaled only when the
-// maximum has grown by more than 8 in base 2 (the weights stay below 2^8),
-// which after the first steps is rare; the result does not depend on m but
-// for rounding.
+// maximum has grown by more than 8 in base 2 (the weights stay below 2^8, or
+// 2^15 in half, see kLift), which after the first steps is rare; the result
+// does not depend on m but for rounding.
 //
 // Roles: warps 0-3 and 4-7 softmax and output of the two tiles, warp 8 issues
 // the products with K, warp 10 those with V, warp 9 the copies (11 only fills
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_put32(tO + c, u);
                 }
             }
-            const float ref = m == -INFINITY ? 0.f : -m * sc;
+            const float ref = (m == -INFINITY ? 0.f : -m * sc) + kLift<T>;
             const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
             float2 add = make_float2(0.f, 0.f);
 #pragma unroll
