@@ -515,7 +515,8 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
  * 32, 64 or 128, n_in a multiple of it; x and out of `dtype` (F32, F16 or
  * BF16), rows x_stride and out_stride values apart, w and the rows of x
  * 16-byte aligned; bias F32 or NULL; at most 524280 rows, n_out and n_in at
- * most 2^31 - 65536. Products are exact and sums 32-bit. A
+ * most 2^31 - 65536. Products are exact (F32 x: from 2^-115 in magnitude on)
+ * and sums 32-bit. A
  * bounded wait that ran out is reported as above. */
 int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in, int32_t group, const uint8_t *w,
                         const uint16_t *scales, int32_t dtype, const void *x, int64_t x_stride, const float *bias,

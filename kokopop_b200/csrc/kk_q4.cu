@@ -3,7 +3,11 @@
 // q in [0, 15], two to a byte (element 2 i in the low nibble of byte i), s
 // half, x and out of one type. Sums are 32-bit; the products are exact:
 // q - 8 fits the 16-bit types, and a 32-bit x is split into three bfloat16
-// parts (8 + 8 + 8 significant bits, its whole range).
+// parts (8 + 8 + 8 significant bits, its whole range). Bfloat16 weights are
+// unpacked as (q - 8) 2^-11 and the scales multiplied by 2^11, so that a
+// group's sum of up to 128 x 8 times the largest x stays finite until its
+// scale is applied. (The last of 24 bits of an x below 2^-115 then fall below
+// the smallest float.)
 //
 // The weights are read once, n_out n_in / 2 bytes, and bound it, with the
 // unpacking close behind: 7 integer operations for 8 weights. A warp takes 16
@@ -99,8 +103,14 @@ __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&v)[4], __half t) {
 __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&v)[4], __nv_bfloat16 t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        v[i] = fma2(mask_or(w >> (4 * i), 0x000f000fu, 0x43004300u), 0x3f803f80u, 0xc308c308u, t);  // 1, -136
+        v[i] = fma2(mask_or(w >> (4 * i), 0x000f000fu, 0x43004300u), 0x3a003a00u, 0xbd88bd88u, t);  // 2^-11 (1, -136)
 }
+
+// a weight over its unpacked value
+template <typename M>
+constexpr float kUnpacked = 2048.f;
+template <>
+constexpr float kUnpacked<__half> = 1.f;
 
 // The type multiplied for x of type T, and the parts of one value.
 template <typename T>
@@ -152,7 +162,7 @@ __device__ __forceinline__ void put(float v, __nv_bfloat16 *p) { *p = __float2bf
 // of the block, w8 its row; x: the lane's 16 bytes of the first 32 k for each
 // tile of rows, x_group and x_part bytes further for the next 32 k and the
 // next part (0 where the lane's row does not exist: it then stays on 16 bytes
-// of zeros); fa: the scales of outputs gid and gid + 8.
+// of zeros); fa: the scales of outputs gid and gid + 8, times kUnpacked.
 template <typename M, int NB, int PARTS, int PG>
 __device__ __forceinline__ void q4_block(uint32_t at, uint32_t w8, const uint32_t (&x0)[NB],
                                          const uint32_t (&x_group)[NB], const uint32_t (&x_part)[NB],
@@ -322,8 +332,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, (Q4Cfg<T, NB, WR>::CTAS))
                 const int s0 = blk * NS;
 #pragma unroll
                 for (int g = 0; g < NS; ++g) {
-                    fa[0][g] = s0 + g < groups ? __half2float(__ldg(sa + s0 + g)) : 0.f;
-                    fa[1][g] = s0 + g < groups ? __half2float(__ldg(sb + s0 + g)) : 0.f;
+                    fa[0][g] = s0 + g < groups ? kUnpacked<M> * __half2float(__ldg(sa + s0 + g)) : 0.f;
+                    fa[1][g] = s0 + g < groups ? kUnpacked<M> * __half2float(__ldg(sb + s0 + g)) : 0.f;
                 }
                 ok = __all_sync(0xffffffffu, mbar_wait_tight(bar, phase, a.err, kErrQ4Wait));
                 if (ok) q4_block<M, NB, PARTS, PG>(at, gid * 16, x, x_group, x_part, fa, acc);

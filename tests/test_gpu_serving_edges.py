@@ -4,7 +4,7 @@ tolerances as in test_gpu_serving.py unless a test says otherwise."""
 import numpy as np
 import pytest
 
-from test_gpu_serving import _attend_plain, _attend_run, _attend_setup
+from test_gpu_serving import DT, KK, UNIT, _attend_plain, _attend_run, _attend_setup, _stream
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,53 @@ def test_attention_rounds_small_weights_as_finely_as_large_ones_in_half(ctx, n, 
     steps = keys // tops // 16
     tol = 2.0 ** -10 + 17 * steps * 2.0 ** -24 + (steps * 2.0 ** -24 if new == 1 else 0.0)
     assert (np.abs(got / want - 1.0) <= tol).all(), (float(np.abs(got / want - 1.0).max()), tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 9])
+def test_q4_product_of_the_largest_values_is_finite_where_the_definition_is(ctx, dtype, rows):
+    """A group's sum of x (q - 8) can pass the largest float although its
+    product with the scale does not."""
+    n_out, n_in, group = 40, 256, 128
+    big = torch.finfo(DT[dtype]).max
+    x = torch.full((rows, n_in), big, device="cuda").to(DT[dtype])
+    x[:, 1::3] *= -0.25
+    x[:, group:] *= 2.0 ** -20
+    w = torch.zeros(n_out, n_in // 2, dtype=torch.uint8, device="cuda")  # every weight -8
+    w[1::2] = 0xff                                                       # or 7
+    sc = torch.full((n_out, n_in // group), 2.0 ** -11, device="cuda").half()
+    out = torch.empty(rows, n_out, dtype=DT[dtype], device="cuda")
+    ctx.q4_matvec_device(rows, n_out, n_in, group, w.data_ptr(), sc.data_ptr(), KK[dtype], x.data_ptr(), n_in, 0,
+                         out.data_ptr(), n_out, _stream())
+    torch.cuda.synchronize()
+    q = torch.full((n_out, n_in), -8.0, dtype=torch.float64, device="cuda")
+    q[1::2] = 7.0
+    q *= 2.0 ** -11
+    want, size = x.double() @ q.T, x.double().abs() @ q.abs().T
+    assert float(want.abs().max()) < torch.finfo(torch.float32).max
+    tol = (n_in + 4) * 2.0 ** -23 * size + UNIT[dtype] * want.abs()
+    assert bool(((out.double() - want).abs() <= tol).all())
+
+
+def test_q4_product_of_small_values_keeps_their_bits(ctx):
+    """F32 rows around 2^-100: nothing but the 32-bit sums rounds, apart from
+    what of a product of an x below 2^-115 is below the smallest float (2^-149,
+    2^11 times that in the result, times the scale)."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    rows, n_out, n_in, group = 3, 70, 640, 64
+    x = torch.randn(rows, n_in, device="cuda", generator=g) * 2.0 ** -100
+    w = torch.randint(0, 256, (n_out, n_in // 2), dtype=torch.uint8, device="cuda", generator=g)
+    sc = torch.rand(n_out, n_in // group, device="cuda", generator=g).half()
+    out = torch.empty(rows, n_out, device="cuda")
+    ctx.q4_matvec_device(rows, n_out, n_in, group, w.data_ptr(), sc.data_ptr(), KK["f32"], x.data_ptr(), n_in, 0,
+                         out.data_ptr(), n_out, _stream())
+    torch.cuda.synchronize()
+    q = torch.empty(n_out, n_in, dtype=torch.float64, device="cuda")
+    q[:, 0::2], q[:, 1::2] = (w.long() % 16 - 8).double(), (w.long() // 16 - 8).double()
+    q *= sc.double().repeat_interleave(group, dim=1)
+    want, size = x.double() @ q.T, x.double().abs() @ q.abs().T
+    tol = (n_in + 4) * 2.0 ** -23 * size + 3 * n_in * 2.0 ** -138
+    assert bool(((out.double() - want).abs() <= tol).all())
+    rel = float((out.double() - want).norm(dim=1).div(want.norm(dim=1)).max())
+    assert rel <= n_in ** 0.5 * 2.0 ** -23, rel
