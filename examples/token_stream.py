@@ -136,6 +136,7 @@ class TokenStream:
         for _ in range(steps):
             logits.append(self.step(out[-1], one, 1))
             out.append(logits[-1].argmax(-1))
+        self.ctx.serving_status(torch.cuda.current_stream().cuda_stream or kb.STREAM_LEGACY)
         return torch.stack(out, dim=1), torch.stack(logits, dim=1)
 
     def close(self):

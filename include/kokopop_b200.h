@@ -500,8 +500,7 @@ int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_t
  * pieces joined through a workspace of the context: such a call is ordered
  * after the context's previous call, like the other entry points. While the
  * stream is being captured the keys are not divided. Every wait inside is
- * bounded; one that ran out is reported (KK_ERROR_INFERENCE) by the next call
- * of the context that synchronises. */
+ * bounded; kk_serving_status tells of one that ran out. */
 int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t n_seqs, const int32_t *seq_len,
                               const int32_t *cu_new, int64_t n_tokens, int32_t max_new, int32_t max_len,
                               const int32_t *table, int32_t max_pages, const void *q, int64_t q_stride,
@@ -517,10 +516,20 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
  * 16-byte aligned; bias F32 or NULL; at most 524280 rows, n_out and n_in at
  * most 2^31 - 65536. Products are exact (F32 x: from 2^-115 in magnitude on)
  * and sums 32-bit. A
- * bounded wait that ran out is reported as above. */
+ * bounded wait that ran out is told by kk_serving_status. */
 int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in, int32_t group, const uint8_t *w,
                         const uint16_t *scales, int32_t dtype, const void *x, int64_t x_stride, const float *bias,
                         void *out, int64_t out_stride, void *stream);
+
+/* Waits for `stream` and tells whether a bounded wait inside a serving call
+ * of the context (on any stream, captured ones included) has run out since
+ * the last report: KK_OK, or KK_ERROR_INFERENCE with the operator in
+ * kk_last_error(), once for all of them. The outputs of the calls since the
+ * last KK_OK are then not to be used. The calls above are asynchronous and
+ * report nothing themselves, and the synthesis calls report only their own
+ * failures: ask where a step's result is read. Not while the stream is being
+ * captured. */
+int kk_serving_status(kk_ctx *ctx, void *stream);
 
 /* kk_istft without any device allocation (no counterpart in the reference,
  * whose iSTFT runs on the host). Same arguments and results as kk_istft, but
@@ -611,6 +620,10 @@ int kk_inject_allocation_failures(int32_t n);
  * kk_last_error(): the path a real expiry takes (the kernel gives up and
  * returns, the host reports it); the context stays usable. */
 int kk_wait_selftest(kk_ctx *ctx, int64_t limit_us);
+
+/* The same with the bounded wait of the serving operators, asynchronous on
+ * `stream` like they are: kk_serving_status then reports it. */
+int kk_serving_wait_selftest(kk_ctx *ctx, int64_t limit_us, void *stream);
 
 #ifdef __cplusplus
 }

@@ -192,6 +192,8 @@ def load_library():
     L.kk_paged_attention_device.argtypes = [vp, cachep, i32, vp, vp, i64, i32, i32, vp, i32, vp, i64, i32,
                                             ctypes.c_float, i32, vp, i64, vp]
     L.kk_q4_matvec_device.argtypes = [vp, i64, i32, i32, i32, vp, vp, i32, vp, i64, vp, vp, i64, vp]
+    L.kk_serving_status.argtypes = [vp, vp]
+    L.kk_serving_wait_selftest.argtypes = [vp, i64, vp]
     i64p = ctypes.POINTER(ctypes.c_int64)
     cfgp = ctypes.POINTER(StreamConfig)
     L.kk_stream_preset.argtypes = [ctypes.c_int32, cfgp]
@@ -458,6 +460,11 @@ class Context:
         """kk_q4_matvec_device: x [n_rows, n_in], out [n_rows, n_out] of `dtype`; bias_ptr 0: none."""
         self._check(self.L.kk_q4_matvec_device(self.h, n_rows, n_out, n_in, group, w_ptr, scales_ptr, dtype, x_ptr,
                                                x_stride, bias_ptr, out_ptr, out_stride, stream))
+
+    def serving_status(self, stream: int = 0) -> None:
+        """kk_serving_status: waits for the stream; raises KKError if a wait
+        inside a serving call ran out since the last report."""
+        self._check(self.L.kk_serving_status(self.h, stream))
 
     # ---- LSTM stack and durations ----
 

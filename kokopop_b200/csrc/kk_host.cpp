@@ -178,10 +178,12 @@ float *kk_ctx::buf(const char *name, size_t floats) {
     return (float *)b.p;
 }
 
-// The device status block: error word 0, no non-finite index recorded.
+// The device status block: error word 0, no non-finite index recorded. The
+// serving operators' word is left: it is theirs to report and to clear.
 void kk_ctx::reset_status() {
     d_err.ensure(sizeof(DevStatus));
-    check_cuda(cudaMemset(d_err.p, 0, offsetof(DevStatus, first)), "clear status");
+    check_cuda(cudaMemset(d_err.p, 0, offsetof(DevStatus, serving)), "clear status");
+    check_cuda(cudaMemset((char *)d_err.p + offsetof(DevStatus, sched), 0, sizeof(DevStatus::sched)), "clear status");
     check_cuda(cudaMemset((char *)d_err.p + offsetof(DevStatus, first), 0xff, sizeof(DevStatus::first)),
                "clear status");
 }
@@ -2025,10 +2027,6 @@ void check_device_error(kk_ctx *ctx) {
     if (e == kErrLstmWait)
         throw KKError(KK_ERROR_INFERENCE, "LSTM recurrence timed out waiting for a step's hidden state (code " +
                                               std::to_string(e) + ")");
-    if (e == kErrPagedWait)
-        throw KKError(KK_ERROR_INFERENCE, "paged attention timed out waiting (code " + std::to_string(e) + ")");
-    if (e == kErrQ4Wait)
-        throw KKError(KK_ERROR_INFERENCE, "4-bit product timed out waiting (code " + std::to_string(e) + ")");
     throw KKError(KK_ERROR_INFERENCE, "tensor-core convolution timed out waiting (code " + std::to_string(e) + ")");
 }
 
@@ -2064,6 +2062,8 @@ int kk_ctx_create(int device, kk_ctx **out) {
         for (auto &s : c->stage) check_cuda(cudaEventCreateWithFlags(&s.ev, cudaEventDisableTiming), "event");
         check_cuda(conv_simt_init(), "conv init");
         c->reset_status();
+        check_cuda(cudaMemset(c->serving_err(), 0, sizeof(int)), "clear serving status");
+        check_cuda(cudaStreamSynchronize(nullptr), "clear status");  // the streams here do not wait for this one
         *out = c.release();
         return KK_OK;
     });

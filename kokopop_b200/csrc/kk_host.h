@@ -173,6 +173,7 @@ struct kk_ctx {
     std::unordered_map<std::string, kk::DevBuf> adain_t;  // fc weights transposed to [128][C]
     kk::DevBuf d_err;  // device status block (kk::DevStatus): error word, non-finite indices
     void reset_status();
+    int *serving_err() { return (int *)((char *)d_err.p + offsetof(kk::DevStatus, serving)); }
     kk::SineArgs sine{};
     std::vector<kk::SiteInfo> sites;
     std::unordered_map<std::string, int> site_index;

@@ -251,7 +251,7 @@ enum { kFiniteF0 = 0, kFiniteNoise, kFiniteAsr, kFiniteDecoder, kFiniteStyle, kF
 constexpr int kErrNonFinite = 60;  // + label
 struct DevStatus {
     int code;
-    int pad;
+    int serving;  // error word of the serving operators (kk_serving_status)
     // the dynamic tile order of the channels x positions convolution: the
     // next tile past the static first ones, and the CTAs done (both zero
     // between launches: the last CTA of a launch resets them)
@@ -267,6 +267,8 @@ constexpr int kErrWaitSelftest = 77;
 // The LSTM recurrence's wait for a step's hidden state ran out (1 s).
 constexpr int kErrLstmWait = 45;
 cudaError_t wait_selftest(int *err, unsigned long long limit_ns, cudaStream_t st);
+// The same with the wait of the serving operators (mbar_wait_tight).
+cudaError_t wait_tight_selftest(int *err, unsigned long long limit_ns, cudaStream_t st);
 // pos / type non-null (ALBERT): + the position row t and the token type row 0
 void embed(const float *emb, int C, int vocab, const int32_t *ids, const int64_t *cum, const Batch &b, float *X,
            int64_t R, int *err, cudaStream_t st, const float *pos = nullptr, const float *type = nullptr);
@@ -408,7 +410,7 @@ struct PagedAttnArgs {
     float2 *part_ml; // [n_tokens][n_heads][splits] running maximum (base 2) and sum
     unsigned *count; // row kernel: [tiles][n_kv_heads], zero between launches
     int *part_n;     // chunk kernel: [n_tokens][n_heads], pieces of a row
-    int *err;        // device error word
+    int *err;        // device error word (DevStatus::serving)
 };
 // How a call is divided: the tensor-memory kernel (chunks of queries) or the
 // row kernel (a few queries of each request), rows (query, head of the group)
@@ -426,7 +428,7 @@ cudaError_t paged_attn(const PagedAttnPlan &p, const PagedAttnArgs &a, cudaStrea
 bool paged_chunk_serves(const PagedCacheView &c, int n_heads);
 int paged_chunk_unit(int group);
 cudaError_t paged_chunk_attn(const PagedAttnArgs &a, cudaStream_t st);
-// A wait of the chunk kernel ran out (2 s).
+// A wait of one of the attention kernels ran out (2 s).
 constexpr int kErrPagedWait = 78;
 
 // kk_q4.cu
@@ -441,7 +443,7 @@ struct Q4MatvecArgs {
     const float *bias;  // may be null
     void *out;
     int64_t out_stride;
-    int *err;  // device error word
+    int *err;  // device error word (DevStatus::serving)
 };
 // A wait of the 4-bit product for its weights ran out (2 s).
 constexpr int kErrQ4Wait = 79;

@@ -217,7 +217,7 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         a.part_ml = nullptr;
         a.count = nullptr;
         a.part_n = nullptr;
-        a.err = (int *)ctx->d_err.p;
+        a.err = ctx->serving_err();
         // pieces of the key axis
         const int64_t rows = std::min<int64_t>(n_tokens, std::max(max_new, 1)) * group;
         // (all rows are in some tile, whatever max_new says)
@@ -291,9 +291,40 @@ int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in
         a.bias = bias;
         a.out = out;
         a.out_stride = out_stride;
-        a.err = (int *)ctx->d_err.p;
+        a.err = ctx->serving_err();
         check_cuda(q4_matvec(a, stream_of(ctx, stream)), "4-bit product launch");
         ++ctx->n_launches;
+        return KK_OK;
+    });
+}
+
+int kk_serving_status(kk_ctx *ctx, void *stream) {
+    return guarded([&] {
+        need(ctx != nullptr, "null argument");
+        use_device(ctx);
+        cudaStream_t st = stream_of(ctx, stream);
+        need(!capturing(st), "the stream is being captured");
+        int code = 0;
+        check_cuda(cudaMemcpyAsync(&code, ctx->serving_err(), sizeof code, cudaMemcpyDeviceToHost, st),
+                   "read serving status");
+        check_cuda(cudaStreamSynchronize(st), "serving operators");
+        if (code == 0) return KK_OK;
+        check_cuda(cudaMemsetAsync(ctx->serving_err(), 0, sizeof code, st), "clear serving status");
+        check_cuda(cudaStreamSynchronize(st), "clear serving status");
+        const std::string c = " (code " + std::to_string(code) + ")";
+        if (code == kErrPagedWait) throw KKError(KK_ERROR_INFERENCE, "paged attention timed out waiting" + c);
+        if (code == kErrQ4Wait) throw KKError(KK_ERROR_INFERENCE, "4-bit product timed out waiting" + c);
+        throw KKError(KK_ERROR_INFERENCE, "bounded wait ran out, self-test" + c);
+    });
+}
+
+int kk_serving_wait_selftest(kk_ctx *ctx, int64_t limit_us, void *stream) {
+    return guarded([&] {
+        need(ctx && limit_us >= 1 && limit_us <= 2000000, "bad argument");
+        use_device(ctx);
+        check_cuda(wait_tight_selftest(ctx->serving_err(), (unsigned long long)limit_us * 1000ull,
+                                       stream_of(ctx, stream)),
+                   "wait self-test launch");
         return KK_OK;
     });
 }

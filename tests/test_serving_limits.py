@@ -31,3 +31,11 @@ def test_sizes_whose_indices_pass_32_bits_are_refused(call, bad):
 def test_arrays_that_are_not_aligned_to_their_type_are_refused(call, bad):
     assert call(**bad) == kb.KK_ERROR_INVALID_ARGUMENT
     assert "aligned" in kb.load_library().kk_last_error().decode()
+
+
+def test_status_and_its_self_test_refuse_bad_arguments():
+    L = kb.load_library()
+    for rc in (L.kk_serving_status(None, None), L.kk_serving_wait_selftest(None, 1000, None),
+               L.kk_serving_wait_selftest(P, 0, None), L.kk_serving_wait_selftest(P, 2000001, None)):
+        assert rc == kb.KK_ERROR_INVALID_ARGUMENT
+        assert L.kk_last_error().decode()
