@@ -414,11 +414,13 @@ struct PagedAttnArgs {
 };
 // How a call is divided: the tensor-memory kernel (chunks of queries) or the
 // row kernel (a few queries of each request), rows (query, head of the group)
-// of a tile, and at most how many tiles there are.
+// of a tile, at most how many tiles there are, and at most how many requests
+// have new tokens if the largest number of them is max_new (the others of the
+// n_seqs are idle).
 struct PagedAttnPlan {
     bool chunk;
     int unit;
-    int64_t tiles;
+    int64_t tiles, busy;
 };
 // keys: at most that many are seen by a query.
 PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new,

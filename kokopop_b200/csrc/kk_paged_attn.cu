@@ -535,9 +535,12 @@ static cudaError_t launch_row_of(const PagedAttnPlan &p, const PagedAttnArgs &a,
 PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new,
                               int64_t keys) {
     const int group = n_heads / c.n_kv_heads;
-    const int64_t rows = (n_tokens < max_new ? n_tokens : max_new) * (int64_t)group;
-    const bool short_rows = rows <= 48 && keys <= 1024 && (int64_t)n_seqs * c.n_kv_heads >= 2 * 148;
+    const int64_t most = n_tokens < max_new ? n_tokens : max_new, rows = most * group;
+    // one request has `most` new tokens, each other busy one at least one
+    const int64_t others = n_tokens - (most > 0 ? most : 1);
     PagedAttnPlan p;
+    p.busy = others + 1 < n_seqs ? others + 1 : n_seqs;
+    const bool short_rows = rows <= 48 && keys <= 1024 && p.busy * c.n_kv_heads >= 2 * 148;
     p.chunk = rows > kFewRows && !short_rows && paged_chunk_serves(c, n_heads);
     p.unit = p.chunk ? paged_chunk_unit(group) : rows > 8 ? 16 : 8;
     p.tiles = n_tokens * group / p.unit + n_seqs;

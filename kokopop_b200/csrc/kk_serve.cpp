@@ -223,7 +223,9 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
         // (all rows are in some tile, whatever max_new says)
         const int64_t least = (n_tokens * group + plan.unit - 1) / plan.unit;
         const int64_t blocks =
-            std::max(least, std::min(plan.tiles, n_seqs * ((rows + plan.unit - 1) / plan.unit))) * a.cache.n_kv_heads;
+            std::max(least, std::min(plan.tiles - n_seqs + plan.busy,  // idle slots have no block
+                                     plan.busy * ((rows + plan.unit - 1) / plan.unit))) *
+            a.cache.n_kv_heads;
         if (window > 0) keys = std::min<int64_t>(std::max(max_len, 1), (int64_t)window + plan.unit / group + 16);
         a.splits = capturing(st) ? 1 : plan.chunk ? chunk_pieces(blocks, keys) : row_pieces(blocks, keys);
         const int64_t step = plan.chunk ? 128 : 64;

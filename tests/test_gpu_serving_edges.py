@@ -104,3 +104,16 @@ def test_q4_product_of_small_values_keeps_their_bits(ctx):
     assert bool(((out.double() - want).abs() <= tol).all())
     rel = float((out.double() - want).norm(dim=1).div(want.norm(dim=1)).max())
     assert rel <= n_in ** 0.5 * 2.0 ** -23, rel
+
+
+@pytest.mark.parametrize("new,slots,at", [(1, 64, 37), (70, 64, 0), (70, 300, 299)])
+def test_idle_slots_do_not_change_the_division_of_the_keys(ctx, new, slots, at):
+    """A request alone and the same one among slots without new tokens (some
+    with keys in the cache): one division of its keys, so the same bits."""
+    k, v, table, q = _attend_setup([5000], [new], 8, 2, 64, 16, "token", "bf16")
+    alone = _attend_run(ctx, k, v, table, [5000], [new], q, 8, 0.125, 0, "bf16")
+    lens, news = [i % 2 * 40 for i in range(slots)], [0] * slots
+    lens[at], news[at] = 5000, new
+    many = np.repeat(table, slots, axis=0)
+    got = _attend_run(ctx, k, v, many, lens, news, q, 8, 0.125, 0, "bf16")
+    np.testing.assert_array_equal(got, alone)
