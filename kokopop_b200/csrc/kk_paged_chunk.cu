@@ -420,9 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         const int n = x ? n_step[1] : n_step[0];
         // whether a page of the block's keys is missing, looked up while the
-        // first copies are under way; without a step there is no page to look up
+        // first copies are under way (k0 is at most the table's end: without a
+        // key the loop reads nothing, or a column of the table)
         bool gone = false;
-        for (int64_t key = k0 / page_size * page_size + (int64_t)tid * page_size; steps > 0 && key < k1;
+        for (int64_t key = k0 / page_size * page_size + (int64_t)tid * page_size; key < k1;
              key += (int64_t)2 * kTile * page_size) {
             const int page = table[(int)key / page_size];
             gone |= page < 0 || page >= a.cache.n_pages;
@@ -492,7 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_put32(tO + c, u);
                 }
             }
-            const float ref = (m == -INFINITY ? 0.f : -m * sc) + kLift<T>;
+            float ref = m == -INFINITY ? 0.f : -m * sc;
+            if constexpr (kLift<T> != 0.f) ref += kLift<T>;  // an addition of 0 would stay in the code
             const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
             float2 add = make_float2(0.f, 0.f);
 #pragma unroll
