@@ -69,24 +69,30 @@ bool capturing(cudaStream_t st) {
 
 // Pieces of the key axis for the chunk kernel: the number that gives the
 // shortest time of whole rounds of 148 blocks, a block's start and end costing
-// about 3 of its steps of 128 keys (7000 + 3000 clocks against 4000) and the
-// join as much again.
+// as much as kPieceEnds of its steps of 128 keys (1.6 us each) and the join
+// with its traffic as much as kJoinSteps. Both are fitted to a sweep on B200:
+// 8 to 448 blocks, 1000 to 30000 keys, heads of 64 and of 128, 1 to 64 pieces.
+// With them the chosen number is 1 % slower than the best one on average and
+// 13 % at most; with 3 and 3 6 % and 46 % (200 blocks over 2000 keys: 117 us in
+// two pieces, 80 in one).
+constexpr int kPieceEnds = 8, kJoinSteps = 8;
 int chunk_pieces(int64_t blocks, int64_t keys) {
     const int64_t most = std::min<int64_t>((keys + 255) / 256, 64);
     int best = 1;
     int64_t best_cost = INT64_MAX;
     for (int64_t s = 1; s <= most; ++s) {
         const int64_t steps = (keys + 128 * s - 1) / (128 * s);
-        const int64_t cost = (blocks * s + 147) / 148 * (steps + 3) + (s > 1 ? 3 : 0);
+        const int64_t cost = (blocks * s + 147) / 148 * (steps + kPieceEnds) + (s > 1 ? kJoinSteps : 0);
         if (cost < best_cost) best = (int)s, best_cost = cost;
     }
     return best;
 }
 
 // For the row kernel: about two blocks for each of the two places on an SM,
-// 256 keys or more each. Measured on B200 at 296, 592, 1184, 2368 blocks:
-// 64 requests of 17-4099 keys 122, 108, 106, 113 us; 7 of 30011-65000 keys
-// 232, 231, 246, 241 us.
+// 256 keys or more each. Measured on B200 at 148, 296, 592, 888, 1184, 2368
+// blocks, 32 heads on 8, one token each: 64 requests of 17-4099 keys 113, 113,
+// 106, 106, 104, 113 us (heads of 64: 64, 64, 60, 60, 67, 64); 7 of 30011-65000
+// keys 264, 229, 218, 227, 229, 230; one of 65000 51, 52, 57, 64, 67, 84.
 int row_pieces(int64_t blocks, int64_t keys) {
     return (int)std::min<int64_t>(std::min((592 + blocks - 1) / blocks, (keys + 255) / 256), 256);
 }
