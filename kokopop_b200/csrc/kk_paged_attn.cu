@@ -525,13 +525,18 @@ static cudaError_t launch_row_of(const PagedAttnPlan &p, const PagedAttnArgs &a,
 }
 
 // Chunks of queries take the chunk kernel, whose blocks read the keys once for
-// 256 rows but start and end slowly (about 5 us). Up to 48 rows over few keys
-// in many requests, the row kernel's smaller blocks are done sooner although
-// they read the keys up to three times: 105 requests of 18-41 new tokens, 16
-// heads, 41-410 keys 131 us against 157; 80 of 3-4 tokens, 8 heads on each of
-// 4, a window of 487 keys 39 against 52. With less than two rounds of chunk
-// blocks there is nothing to win: 32 requests of 5 tokens, 4 heads on each of 8,
-// 500-2000 keys 76 against 75; 45 of 8-13 tokens, 8 heads on one 38 against 24.
+// 256 rows but start and end slowly (about 5 us). Up to 48 rows over at most
+// 1024 keys in many requests, the row kernel's smaller blocks are done sooner
+// although they read the keys once per 16 rows. Measured on B200, row against
+// chunk kernel, 300 and 1184 pairs of request and key head:
+//   heads of 64   48 rows, 1024 keys 37 / 47 and 110 / 171 us; 17-41 rows, 410
+//                 keys (608 pairs) 29 / 54 us
+//   heads of 128  32 rows, 410 keys (608 pairs) 49 / 62, 1024 keys 80 / 98 us;
+//                 18-41 rows, 30 on average, 1024 keys 88 / 93; 33 rows, 1024
+//                 keys 102 / 93; 48 rows 69 / 52 and 233 / 187 us
+// so that heads above 64 take it up to 32 rows on average. With less than two
+// rounds of chunk blocks it loses: 148 pairs, 20 rows, 300 keys 17 / 15 and
+// (heads of 128) 27 / 17 us.
 PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_tokens, int n_seqs, int max_new,
                               int64_t keys) {
     const int group = n_heads / c.n_kv_heads;
@@ -540,7 +545,8 @@ PagedAttnPlan paged_attn_plan(const PagedCacheView &c, int n_heads, int64_t n_to
     const int64_t others = n_tokens - (most > 0 ? most : 1);
     PagedAttnPlan p;
     p.busy = others + 1 < n_seqs ? others + 1 : n_seqs;
-    const bool short_rows = rows <= 48 && keys <= 1024 && p.busy * c.n_kv_heads >= 2 * 148;
+    const bool short_rows = rows <= 48 && keys <= 1024 && p.busy * c.n_kv_heads >= 2 * 148 &&
+                            (c.head_dim <= 64 || n_tokens * group <= 32 * p.busy);
     p.chunk = rows > kFewRows && !short_rows && paged_chunk_serves(c, n_heads);
     p.unit = p.chunk ? paged_chunk_unit(group) : rows > 8 ? 16 : 8;
     p.tiles = n_tokens * group / p.unit + n_seqs;

@@ -4,7 +4,7 @@ tolerances as in test_gpu_serving.py unless a test says otherwise."""
 import numpy as np
 import pytest
 
-from test_gpu_serving import DT, KK, UNIT, _attend_plain, _attend_run, _attend_setup, _stream
+from test_gpu_serving import DT, KK, UNIT, _attend_check, _attend_plain, _attend_run, _attend_setup, _stream
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +117,14 @@ def test_idle_slots_do_not_change_the_division_of_the_keys(ctx, new, slots, at):
     many = np.repeat(table, slots, axis=0)
     got = _attend_run(ctx, k, v, many, lens, news, q, 8, 0.125, 0, "bf16")
     np.testing.assert_array_equal(got, alone)
+
+
+@pytest.mark.parametrize("new", [(5, 8), (12, 12)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_many_short_requests_on_either_kernel(ctx, dim, new):
+    """Up to 32 rows on average, and 48: heads of 128 change kernels between."""
+    rng = np.random.default_rng(dim)
+    new = rng.integers(new[0], new[1] + 1, 160).tolist()
+    lens = [int(n + rng.integers(0, 60)) for n in new]
+    for window in (0, 20):
+        _attend_check(ctx, lens, new, 8, 2, dim, 16, window, "token", "f16")
