@@ -86,12 +86,16 @@ class PagedCache(ctypes.Structure):
 def q4_pack(w: np.ndarray, group: int):
     """Weights [n_out, n_in] as the 4-bit products take them: bytes [n_out,
     n_in / 2] and half scales [n_out, n_in / group]. A group's scale is its
-    largest magnitude / 7, a weight the nearest q - 8 with q in [1, 15]."""
+    largest magnitude / 7, a weight the nearest q - 8 with q in [1, 15].
+    Weights must be finite and below 7 times half's largest number."""
     w = np.asarray(w, np.float32)
     if w.ndim != 2 or group not in (32, 64, 128) or w.shape[1] % group != 0:
         raise KKError(KK_ERROR_INVALID_ARGUMENT, "weights must be [n_out, n_in] with n_in a multiple of 32, 64 or 128")
     g = w.reshape(w.shape[0], -1, group)
-    scales = (np.abs(g).max(axis=2) / 7.0).astype(np.float16)
+    most = np.abs(g).max(axis=2, initial=0.0) / 7.0
+    if not (most < 65520.0).all():  # from there on half rounds to infinity; a NaN is not below either
+        raise KKError(KK_ERROR_INVALID_ARGUMENT, "weights are not finite, or a scale passes half's largest")
+    scales = most.astype(np.float16)
     s = scales.astype(np.float32)[..., None]
     q = np.where(s > 0, np.rint(np.divide(g, s, out=np.zeros_like(g), where=s > 0)), 0.0)
     q = (np.clip(q, -7, 7) + 8).astype(np.uint8).reshape(w.shape)

@@ -1,5 +1,6 @@
 """Arguments of the serving operators that no kernel could take safely are
 refused before a GPU is touched."""
+import numpy as np
 import pytest
 
 import kokopop_b200 as kb
@@ -39,3 +40,16 @@ def test_status_and_its_self_test_refuse_bad_arguments():
                L.kk_serving_wait_selftest(P, 0, None), L.kk_serving_wait_selftest(P, 2000001, None)):
         assert rc == kb.KK_ERROR_INVALID_ARGUMENT
         assert L.kk_last_error().decode()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 7 * 65520.0, -1e30])
+def test_q4_pack_refuses_weights_that_no_scale_holds(bad):
+    """They would come back as NaN. 7 x 65504 still has a scale."""
+    w = np.ones((3, 64), np.float32)
+    w[1, 40] = 7 * 65504.0
+    q, s = kb.q4_pack(w, 32)
+    assert kb.q4_unpack(q, s, 32)[1, 40] == 7 * 65504.0
+    w[2, 5] = bad
+    with pytest.raises(kb.KKError) as e:
+        kb.q4_pack(w, 32)
+    assert e.value.code == kb.KK_ERROR_INVALID_ARGUMENT
