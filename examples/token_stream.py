@@ -93,7 +93,7 @@ class TokenStream:
         """tokens: the new tokens of all requests, one after another; new: how
         many of each request (int32, on the device). Returns the logits of
         every token."""
-        stream = torch.cuda.current_stream().cuda_stream or kb.STREAM_LEGACY
+        stream = torch.cuda.current_stream(self.device).cuda_stream or kb.STREAM_LEGACY
         t = tokens.shape[0]
         self.longest += max_new
         slots = torch.empty(t, dtype=torch.int64, device=self.device)
@@ -136,11 +136,11 @@ class TokenStream:
         for _ in range(steps):
             logits.append(self.step(out[-1], one, 1))
             out.append(logits[-1].argmax(-1))
-        self.ctx.serving_status(torch.cuda.current_stream().cuda_stream or kb.STREAM_LEGACY)
+        self.ctx.serving_status(torch.cuda.current_stream(self.device).cuda_stream or kb.STREAM_LEGACY)
         return torch.stack(out, dim=1), torch.stack(logits, dim=1)
 
     def close(self):
-        torch.cuda.synchronize()
+        torch.cuda.synchronize(self.device)
         self.ctx.close()
 
 
