@@ -90,24 +90,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
                  : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                                     uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // An 8 x 8 matrix of 16-bit values over the lanes, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t r;
@@ -502,7 +484,7 @@ template <typename T, int DP, int NB, bool TMA>
 static cudaError_t launch_row(const PagedAttnArgs &a, int64_t tiles, cudaStream_t st) {
     static std::atomic<bool> attr[64];
     using C = RowCfg<DP, NB>;
-    cudaError_t e = paged_smem_once(k_paged_attn_row<T, DP, NB, TMA>, C::SMEM, attr);
+    cudaError_t e = dynamic_smem_once(k_paged_attn_row<T, DP, NB, TMA>, C::SMEM, attr);
     if (e != cudaSuccess) return e;
     CUtensorMap mk, mv;
     memset(&mk, 0, sizeof mk);

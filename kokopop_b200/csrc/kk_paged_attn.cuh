@@ -7,8 +7,6 @@
 
 #include <cuda.h>
 
-#include <atomic>
-
 namespace kk {
 
 __device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
@@ -107,20 +105,5 @@ cudaError_t paged_cache_maps(const PagedCacheView &c, int keys, CUtensorMap *k, 
 cudaError_t paged_q_map(const PagedAttnArgs &a, int heads, int tokens, CUtensorMap *m);
 // tensor-map strides are below 2^40 bytes and not 0
 bool paged_strides_mappable(const PagedCacheView &c);
-
-// cudaFuncSetAttribute of the dynamic shared memory, once per device
-template <typename F>
-cudaError_t paged_smem_once(F *kernel, int bytes, std::atomic<bool> (&done)[64]) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!done[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != cudaSuccess) return e;
-        done[dev].store(true, std::memory_order_release);
-    }
-    return cudaSuccess;
-}
 
 }  // namespace kk

@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
 
 static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> g_encode{nullptr};
 
-static cudaError_t encoder(PFN_cuTensorMapEncodeTiled_v12000 *out) {
+cudaError_t tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000 *out) {
     *out = g_encode.load(std::memory_order_acquire);
     if (*out) return cudaSuccess;
     cudaDriverEntryPointQueryResult q;
@@ -620,7 +620,7 @@ static CUtensorMapDataType map_type(int bf16) {
 
 cudaError_t paged_cache_maps(const PagedCacheView &c, int keys, CUtensorMap *k, CUtensorMap *v) {
     PFN_cuTensorMapEncodeTiled_v12000 encode;
-    const cudaError_t e = encoder(&encode);
+    const cudaError_t e = tensor_map_encoder(&encode);
     if (e != cudaSuccess) return e;
     const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv_heads,
                                 (cuuint64_t)c.n_pages};
@@ -638,7 +638,7 @@ cudaError_t paged_cache_maps(const PagedCacheView &c, int keys, CUtensorMap *k, 
 
 cudaError_t paged_q_map(const PagedAttnArgs &a, int heads, int tokens, CUtensorMap *m) {
     PFN_cuTensorMapEncodeTiled_v12000 encode;
-    const cudaError_t e = encoder(&encode);
+    const cudaError_t e = tensor_map_encoder(&encode);
     if (e != cudaSuccess) return e;
     const cuuint64_t dims[3] = {(cuuint64_t)a.cache.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)a.cache.head_dim * 2, (cuuint64_t)a.q_stride * 2};
@@ -664,7 +664,7 @@ int paged_chunk_unit(int group) { return 2 * (kTile / group) * group; }
 template <typename T, int DP>
 static cudaError_t launch_chunk(const PagedAttnArgs &a, cudaStream_t st) {
     static std::atomic<bool> attr[64];
-    cudaError_t e = paged_smem_once(k_paged_attn_chunk<T, DP>, ChunkCfg<DP>::SMEM, attr);
+    cudaError_t e = dynamic_smem_once(k_paged_attn_chunk<T, DP>, ChunkCfg<DP>::SMEM, attr);
     if (e != cudaSuccess) return e;
     const int group = a.n_heads / a.cache.n_kv_heads, tile_tok = kTile / group;
     CUtensorMap q, k, v;

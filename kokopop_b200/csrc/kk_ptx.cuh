@@ -1,10 +1,14 @@
 // Inline PTX of the tensor-core kernels (sm_100a): mbarriers with bounded
-// waits, bulk and tensor copies, tcgen05 and its descriptors.
+// waits, bulk and tensor copies, tcgen05 and its descriptors, mma.sync; and
+// what their launches share.
 #pragma once
 
 #include "kk_common.cuh"
 
 #include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
 
 namespace kk {
 
@@ -85,7 +89,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
         : "memory");
 }
 
-// 2-D tensor copies of one [32 ch][32 rows] F32 block (x = row, y = channel).
+// 2-D tensor copies of one box (x innermost).
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -173,6 +177,43 @@ __device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&r)[32]) {
           "=f"(r[30]), "=f"(r[31])
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Warp-level products of 16-bit values, c += A (16 x 16) B (16 x 8), sums 32-bit.
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                     uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// cuTensorMapEncodeTiled of the driver, looked up once.
+cudaError_t tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000 *out);
+
+// cudaFuncSetAttribute of the dynamic shared memory, once per device
+template <typename F>
+cudaError_t dynamic_smem_once(F *kernel, int bytes, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+        done[dev].store(true, std::memory_order_release);
+    }
+    return cudaSuccess;
 }
 
 }  // namespace kk

@@ -47,29 +47,11 @@ namespace {
 
 constexpr int kQ4Warps = 8;
 
+// mma16 from a sum of 0.
 template <typename T>
-__device__ __forceinline__ void mma_q4(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma_q4<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma_q4<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                                      uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// The same from a sum of 0.
-template <typename T>
-__device__ __forceinline__ void mma_q4_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     c[0] = c[1] = c[2] = c[3] = 0.f;
-    mma_q4<T>(c, a, b0, b1);
+    mma16<T>(c, a, b0, b1);
 }
 
 // The 8 weights of a word as 4 pairs (nibbles i and i + 4) of values q - 8.
@@ -196,10 +178,10 @@ __device__ __forceinline__ void q4_block(uint32_t at, uint32_t w8, const uint32_
 #pragma unroll
             for (int p = PARTS - 1; p >= 0; --p) {
                 if (g % PG == 0 && p == PARTS - 1)
-                    mma_q4_first<M>(c[b], lo, v[b][p][0], v[b][p][1]);
+                    mma16_first<M>(c[b], lo, v[b][p][0], v[b][p][1]);
                 else
-                    mma_q4<M>(c[b], lo, v[b][p][0], v[b][p][1]);
-                mma_q4<M>(c[b], hi, v[b][p][2], v[b][p][3]);
+                    mma16<M>(c[b], lo, v[b][p][0], v[b][p][1]);
+                mma16<M>(c[b], hi, v[b][p][2], v[b][p][3]);
             }
         if (g % PG == PG - 1)
 #pragma unroll
@@ -376,20 +358,11 @@ __global__ void __launch_bounds__(kQ4Warps * 32, (Q4Cfg<T, NB, WR>::CTAS))
     }
 }
 
-static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> g_encode{nullptr};
-
 // the weights as bytes, boxes of 128 bytes x 16 outputs, swizzled; outside reads as 0
 static cudaError_t weight_map(const Q4MatvecArgs &a, CUtensorMap *m) {
-    auto encode = g_encode.load(std::memory_order_acquire);
-    if (!encode) {
-        cudaDriverEntryPointQueryResult q;
-        void *fn = nullptr;
-        cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q);
-        if (e != cudaSuccess) return e;
-        if (q != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
-        encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
-        g_encode.store(encode, std::memory_order_release);
-    }
+    PFN_cuTensorMapEncodeTiled_v12000 encode;
+    const cudaError_t e = tensor_map_encoder(&encode);
+    if (e != cudaSuccess) return e;
     const cuuint64_t dims[2] = {(cuuint64_t)a.n_in / 2, (cuuint64_t)a.n_out};
     const cuuint64_t strides[1] = {(cuuint64_t)a.n_in / 2};
     const cuuint32_t box[2] = {128, 16}, step[2] = {1, 1};
@@ -403,16 +376,9 @@ static cudaError_t weight_map(const Q4MatvecArgs &a, CUtensorMap *m) {
 template <typename T, int NB, int WR>
 static cudaError_t launch_q4(const Q4MatvecArgs &a, cudaStream_t st) {
     using C = Q4Cfg<T, NB, WR>;
-    static std::atomic<bool> done[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    static std::atomic<bool> attr[64];
+    cudaError_t e = dynamic_smem_once(k_q4_matvec<T, NB, WR>, C::SMEM, attr);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!done[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(k_q4_matvec<T, NB, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-        if (e != cudaSuccess) return e;
-        done[dev].store(true, std::memory_order_release);
-    }
     CUtensorMap m;
     e = weight_map(a, &m);
     if (e != cudaSuccess) return e;
