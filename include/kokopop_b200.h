@@ -499,7 +499,9 @@ int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_t
  * Where there are too few rows for the GPU, the keys are divided and the
  * pieces joined through a workspace of the context: such a call is ordered
  * after the context's previous call, like the other entry points. While the
- * stream is being captured the keys are not divided. Every wait inside is
+ * stream is being captured the keys are not divided, which costs time where
+ * requests x key heads are fewer than the GPU's SMs and caches are long (7
+ * requests of 30011-65000 tokens, 8 key heads: 686 us against 211). Every wait inside is
  * bounded; kk_serving_status tells of one that ran out. */
 int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t n_seqs, const int32_t *seq_len,
                               const int32_t *cu_new, int64_t n_tokens, int32_t max_new, int32_t max_len,

@@ -33,6 +33,7 @@
 // Measured on B200, 32 heads of 128 on 8, one token each: 7 requests of
 // 30011-65000 keys 216 us, 6.8 TB/s of cache read (the copy rate is 6.55); 64
 // requests of 17-4099 keys 97 us, 5.3 TB/s, where blocks start and end unevenly.
+// In one piece, as under capture, the long ones take 686 us: 56 blocks.
 #include "kk_paged_attn.cuh"
 #include "kk_ptx.cuh"
 

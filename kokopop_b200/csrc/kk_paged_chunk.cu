@@ -32,7 +32,8 @@
 // 32 heads of 128 on 8, 476 GFLOP under the masks: 444 us, 1.07 PFLOP/s, in
 // short loops (0.65 of the measured burst rate), 495 us, 0.96 PFLOP/s, in long
 // ones at the power limit (0.70 of the sustained rate). The softmax bounds it:
-// without its exponentials 390 us in short loops.
+// without its exponentials 385 us in short loops. Head dims between 64 and 128
+// cost what 128 does: both products run over the padded tile.
 #include "kk_paged_attn.cuh"
 #include "kk_ptx.cuh"
 

@@ -9,8 +9,8 @@
 // scale is applied. (The last of 24 bits of an x below 2^-115 then fall below
 // the smallest float.)
 //
-// The weights are read once, n_out n_in / 2 bytes, and bound it, with the
-// unpacking close behind: 7 integer operations for 8 weights. A warp takes 16
+// The weights are read once, n_out n_in / 2 bytes, but their unpacking bounds
+// it: 7 integer operations for 8 weights and its latencies. A warp takes 16
 // outputs as the M side of mma.sync.m16n8k16 and 8 or 16 rows of x as its N
 // side, so a row more costs no further work on the weights. The order of k
 // within a product is free as long as both sides agree: a lane takes 8
@@ -27,9 +27,9 @@
 // latter are joined in shared memory, in the order of the warps.
 //
 // Measured on B200, 8192 -> 24576, groups of 128, bfloat16: one row 35 us (3.0
-// TB/s), 8 rows 43 us, 16 rows 66 us. 24 instructions a word of weights, the
-// integer pipe half busy: the unpacking and its latencies bound it, not the
-// bytes (16 us).
+// TB/s), 8 rows 43 us, 16 rows 66 us, and 391 us for 128, each 16 rows reading
+// and unpacking the weights again. 25, 29 and 35 instructions a word of weights,
+// the integer pipe half busy; the bytes alone are 16 us.
 #include "../../include/kokopop_b200.h"
 #include "kk_common.cuh"
 #include "kk_kernels.h"
