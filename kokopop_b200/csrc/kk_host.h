@@ -260,13 +260,14 @@ inline void use_device(kk_ctx *ctx) { check_cuda(cudaSetDevice(ctx->device), "cu
 
 // Brackets one entry point's work on `st`: orders it after the context's
 // previous call, which may have run on another stream and whose workspaces
-// this call reuses, and opens a pinned staging slot for its small uploads.
+// this call reuses, and opens a pinned staging slot for its small uploads
+// (uploads false: there are none, and the host need not wait for a slot).
 struct CallScope {
     kk_ctx &c;
     cudaStream_t st;
-    CallScope(kk_ctx &ctx, cudaStream_t s) : c(ctx), st(s) {
+    CallScope(kk_ctx &ctx, cudaStream_t s, bool uploads = true) : c(ctx), st(s) {
         if (c.done_recorded) check_cuda(cudaStreamWaitEvent(st, c.ev_done, 0), "order after the previous call");
-        c.stage_begin();
+        if (uploads) c.stage_begin();
     }
     ~CallScope() {
         c.done_recorded = cudaEventRecord(c.ev_done, st) == cudaSuccess;

@@ -242,7 +242,7 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
             ++ctx->n_launches;
             return KK_OK;
         }
-        CallScope call_scope(*ctx, st);
+        CallScope call_scope(*ctx, st, false);
         const size_t parts = (size_t)n_tokens * n_heads * a.splits;
         a.part_o = ctx->buf("paged_part_o", parts * a.cache.head_dim);
         a.part_ml = (float2 *)ctx->buf("paged_part_ml", parts * 2);
