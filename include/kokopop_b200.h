@@ -501,8 +501,8 @@ int kk_cache_append_device(kk_ctx *ctx, const kk_paged_cache *cache, int64_t n_t
  * after the context's previous call, like the other entry points. While the
  * stream is being captured the keys are not divided, which costs time where
  * requests x key heads are fewer than the GPU's SMs and caches are long (7
- * requests of 30011-65000 tokens, 8 key heads: 686 us against 211). Every wait inside is
- * bounded; kk_serving_status tells of one that ran out. */
+ * requests of 30011-65000 tokens, 8 key heads: 686 us against 211). Every wait
+ * inside is bounded; kk_serving_status tells of one that ran out. */
 int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t n_seqs, const int32_t *seq_len,
                               const int32_t *cu_new, int64_t n_tokens, int32_t max_new, int32_t max_len,
                               const int32_t *table, int32_t max_pages, const void *q, int64_t q_stride,
@@ -517,8 +517,7 @@ int kk_paged_attention_device(kk_ctx *ctx, const kk_paged_cache *cache, int32_t 
  * BF16), rows x_stride and out_stride values apart, w and the rows of x
  * 16-byte aligned; bias F32 or NULL; at most 524280 rows, n_out and n_in at
  * most 2^31 - 65536. Products are exact (F32 x: from 2^-115 in magnitude on)
- * and sums 32-bit. A
- * bounded wait that ran out is told by kk_serving_status. */
+ * and sums 32-bit. A bounded wait that ran out is told by kk_serving_status. */
 int kk_q4_matvec_device(kk_ctx *ctx, int64_t n_rows, int32_t n_out, int32_t n_in, int32_t group, const uint8_t *w,
                         const uint16_t *scales, int32_t dtype, const void *x, int64_t x_stride, const float *bias,
                         void *out, int64_t out_stride, void *stream);
